@@ -112,7 +112,8 @@ int osm_context_synchronize(osm_context* ctx);
  * OSM_PREFILL_BF16 path, whose outputs are then invalid, bit 6 a checked
  * OSM_PREFILL_BF16 call found bit 5 and re-ran on the fp32 path, whose
  * outputs stand, bit 7 an expert-parallel barrier gave up waiting for a
- * rank, whose outputs are then invalid); the count of tokens
+ * rank, whose outputs are then invalid, bit 8 an adapter index past the
+ * table of osm_q4_gemv_lora, taken as no adapter); the count of tokens
  * routed on the exact path. */
 int osm_context_status(osm_context* ctx, uint32_t* status,
                        uint64_t* exact_tokens);
@@ -170,6 +171,51 @@ int osm_q4_gemv_f32(osm_context* ctx, const uint32_t* packed_dev,
                     const float* scales_dev, const float* biases_dev,
                     uint32_t out_dim, uint32_t in_dim, uint32_t group,
                     const float* x_dev, uint32_t tokens, float* y_dev);
+
+/* Element types of the calls that take them. */
+#define OSM_TYPE_F32 0u
+#define OSM_TYPE_BF16 1u
+#define OSM_TYPE_F16 2u
+
+/* A table of low-rank adapters in device memory, one per request or several
+ * requests to one: A [rank][in_dim] and B [out_dim][rank] per adapter, bf16
+ * or fp16, `count` of them a_stride / b_stride elements apart (0: packed). */
+typedef struct {
+  uint32_t count;             /* adapters in the table, at least 1           */
+  uint32_t rank;              /* rows of A, columns of B: 1..128             */
+  uint32_t type;              /* OSM_TYPE_BF16 or OSM_TYPE_F16, of A and B   */
+  uint32_t reserved;          /* 0                                           */
+  const void* a_dev;
+  const void* b_dev;
+  uint64_t a_stride, b_stride;
+  const float* gain_dev;      /* [count] factor of each adapter, or NULL (1) */
+  const uint32_t* ranks_dev;  /* [count] rows of each adapter that count, at
+                                 most rank, or NULL (all); what lies behind
+                                 them is not used                            */
+} osm_lora;
+
+/* No counterpart in the reference (it serves one model as shipped): a Q4
+ * projection shared by all tokens beside the adapters of many requests,
+ *   y[t] = W x[t] + gain[a] B_a (A_a x[t]),   a = adapter_dev[t],
+ * without the second term where a is negative; an index of `count` or more is
+ * taken as none and sets status bit 8.  lora (and adapter_dev) NULL: the
+ * projection alone.  W as for osm_q4_gemv with bf16 scale and bias; group 64,
+ * in_dim a multiple of 64, any out_dim, any number of tokens (the context's
+ * max_tokens does not bound it).  x and y are rows of one type, x_stride and
+ * y_stride elements apart (0: packed); rows and values behind the last one
+ * are neither read nor written, and y must not overlap x.  Sums are held in
+ * fp32, y is rounded once; a token's row depends on no other token's row and
+ * no other adapter.  A row of x with a NaN or an infinity gives non-finite
+ * values in its own y.  The call uses workspace of the context, one block per
+ * stream (grown outside stream capture; a captured call carries its own
+ * memory in the graph), so calls on two streams do not meet. */
+int osm_q4_gemv_lora(osm_context* ctx, const uint32_t* packed_dev,
+                     const uint16_t* scales_bf16_dev,
+                     const uint16_t* biases_bf16_dev, uint32_t out_dim,
+                     uint32_t in_dim, uint32_t group, const void* x_dev,
+                     uint32_t type, uint64_t x_stride, uint32_t tokens,
+                     const osm_lora* lora, const int32_t* adapter_dev,
+                     void* y_dev, uint64_t y_stride);
 
 /* run_vulkan_swiglu_buffers (include/orbi/streammoe/backend/
  * vulkan_swiglu.hpp:26-30): out = silu(gate) * up. */
@@ -374,6 +420,54 @@ int osm_moe_route(osm_layer* layer, const float* x_dev, uint32_t tokens,
  * weight 0, as osm_moe_route does. */
 int osm_moe_route_logits(osm_layer* layer, const float* x_dev, uint32_t tokens,
                          float* logits_dev, uint32_t* ids_dev, float* weights_dev,
+                         float* mass_dev);
+
+/* How experts are chosen from router logits, beyond the softmax top-k of
+ * osm_moe_route. */
+#define OSM_SCORE_SOFTMAX 0u
+#define OSM_SCORE_SIGMOID 1u
+#define OSM_GROUP_MAX 0u      /* a group is worth its best expert            */
+#define OSM_GROUP_TOP2 1u     /* ... the sum of its two best                 */
+typedef struct {
+  uint32_t experts;           /* 1..1024                                     */
+  uint32_t top_k;             /* 1..32, at most the experts of the kept groups */
+  uint32_t score;             /* OSM_SCORE_*                                 */
+  uint32_t groups;            /* 1 (no groups)..32, divides experts          */
+  uint32_t top_groups;        /* groups kept: 1..groups                      */
+  uint32_t group_score;       /* OSM_GROUP_*                                 */
+  uint32_t renormalize;       /* weights / their sum                         */
+  float scale;                /* factor of the weights, after that           */
+  const float* balance_bias_dev; /* [experts] finite, added to the scores for
+                                 the choice alone, or NULL                   */
+} osm_routing;
+
+/* No counterpart in the reference, whose router is softmax top-k.  For each
+ * of `tokens` rows of logits (type OSM_TYPE_*, row_stride elements apart; 0:
+ * packed): scores s = softmax or sigmoid of the logits, choice c = s + bias;
+ * the top_groups groups of largest value, then the top_k experts of largest c
+ * in them, both with ties to the lower index; weights = s of the picks,
+ * divided by their sum (renormalize), times scale.  The picks are those of
+ * 64-bit scores and choices (without a bias, of the logits, which order
+ * experts alike and do not saturate), in falling order of c.  ids_dev [tokens][top_k], weights_dev
+ * [tokens][top_k], mass_dev [tokens] or NULL (the sum of the picks' scores)
+ * are what osm_moe_experts takes.
+ * An expert whose logit is -infinity or its type's lowest finite value is
+ * masked: never chosen, and not counted in its group (a group of masked
+ * experts alone comes after all others).  Where fewer than top_k experts can
+ * be chosen, the lowest-numbered of the others fill the places with weight 0.
+ * A row with a NaN or +infinity gets ids 0, weights 0, mass 0 and sets status
+ * bit 0; a mass of zero gives weights 0 and sets status bit 1. */
+int osm_route_scores(osm_context* ctx, const osm_routing* routing,
+                     const void* logits_dev, uint32_t type,
+                     uint64_t row_stride, uint32_t tokens, uint32_t* ids_dev,
+                     float* weights_dev, float* mass_dev);
+
+/* osm_route_scores on the router logits of a layer (W x plus its logit bias,
+ * by the reference's own arithmetic as in osm_moe_route_logits); experts and
+ * top_k as the layer's, so that osm_moe_experts takes the result. */
+int osm_moe_route_scores(osm_layer* layer, const osm_routing* routing,
+                         const float* x_dev, uint32_t tokens,
+                         uint32_t* ids_dev, float* weights_dev,
                          float* mass_dev);
 
 /* run_qwen_sparse_moe_vulkan_accum (include/orbi/streammoe/model/

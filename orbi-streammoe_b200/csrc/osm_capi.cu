@@ -125,6 +125,15 @@ struct osm_context {
                                     // (OSM_DG_DECODE=0: the mma.sync kernels throughout)
   uint32_t dg_min_tokens = 96;      // ... of at least this many tokens (OSM_DG_MIN_TOKENS;
                                     // below it the mma.sync grouped kernels are faster)
+  // workspace of the calls that need no Scratch: one block per stream, so that
+  // calls on two streams do not meet; an outgrown block stays (queued work may
+  // still use it) until the context goes
+  struct Work {
+    cudaStream_t stream;
+    void* base;
+    size_t bytes;
+  };
+  std::vector<Work> works;
 };
 
 struct osm_slab {
@@ -368,6 +377,62 @@ int ensure_scratch(osm_context* ctx, size_t T, size_t H, size_t E, size_t k, siz
   s.hq = reinterpret_cast<float2*>(b + o_hq);
   return OSM_OK;
 }
+
+// Workspace of one call on the context's stream.  Under stream capture the
+// memory is the graph's own (an allocation and a release node around the
+// call's kernels), so graphs that replay at the same time share nothing;
+// otherwise it is the stream's block.
+struct CallWork {
+  osm_context* ctx;
+  void* p = nullptr;
+  bool in_graph = false;
+  explicit CallWork(osm_context* c) : ctx(c) {}
+  int get(size_t bytes) {
+    if (bytes == 0) return OSM_OK;
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    OSM_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &cap));
+    if (cap != cudaStreamCaptureStatusNone) {
+      OSM_CUDA(ctx, cudaMallocAsync(&p, bytes, ctx->stream));
+      in_graph = true;
+      return OSM_OK;
+    }
+    osm_context::Work* w = nullptr;
+    for (auto& x : ctx->works)
+      if (x.stream == ctx->stream && x.base) w = &x;
+    if (w && w->bytes >= bytes) {
+      p = w->base;
+      return OSM_OK;
+    }
+    // grown by half at least, so that the outgrown blocks stay few and small
+    const size_t want = align_up(std::max(bytes, w ? w->bytes + w->bytes / 2 : bytes), (size_t)1 << 20);
+    void* q = nullptr;
+    if (cudaMalloc(&q, want) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(ctx, OSM_ENOMEM, "workspace allocation failed");
+    }
+    try {
+      if (w) {
+        ctx->retired.push_back(w->base);
+        w->base = q;
+        w->bytes = want;
+      } else {
+        ctx->works.push_back({ctx->stream, q, want});
+      }
+    } catch (...) {
+      cudaFree(q);
+      return fail(ctx, OSM_ENOMEM, "workspace bookkeeping failed");
+    }
+    p = q;
+    return OSM_OK;
+  }
+  int release(int rc) {
+    if (in_graph) {
+      const cudaError_t e = cudaFreeAsync(p, ctx->stream);
+      if (e != cudaSuccess && rc == OSM_OK) return cuda_fail(ctx, e, "workspace release");
+    }
+    return rc;
+  }
+};
 
 bool layout_ok(const osm_expert_layout* L) {
   if (!L || L->group != 64 || L->hidden == 0 || L->inter == 0) return false;
@@ -1046,6 +1111,7 @@ int osm_context_destroy(osm_context* ctx) {
   cudaStreamSynchronize(ctx->stream);
   if (ctx->sc.base) cudaFree(ctx->sc.base);
   for (void* p : ctx->retired) cudaFree(p);
+  for (const auto& w : ctx->works) cudaFree(w.base);
   if (ctx->status_blk) cudaFree(ctx->status_blk);
   for (const ProfRec& r : ctx->recs) {
     cudaEventDestroy(r.a);
@@ -1286,6 +1352,148 @@ int osm_q4_gemv(osm_context* ctx, const uint32_t* packed, const uint16_t* sc,
                    (int)((tokens + osm::kTokGroup - 1) / osm::kTokGroup), ctx->grid_cap,
                    (int)std::min<uint32_t>(tokens, 8), ctx->stream, &ctx->launches);
   return check_launch(ctx, "q4 gemv");
+}
+
+namespace {
+
+size_t type_bytes(uint32_t type) { return type == OSM_TYPE_F32 ? 4 : 2; }
+
+bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
+
+// Checks a routing and fills the fields of `a` that it gives.
+int routing_args(osm_context* ctx, const osm_routing* r, osm::RouteArgs* a) {
+  if (!r) return fail(ctx, OSM_EINVAL, "route scores: null routing");
+  if (r->experts == 0 || r->experts > (uint32_t)osm::kMaxExperts || r->top_k == 0 ||
+      r->top_k > (uint32_t)osm::kMaxTopK)
+    return fail(ctx, OSM_EINVAL, "route scores: 1..1024 experts and top_k 1..32 are supported");
+  if (r->groups == 0 || r->groups > 32 || r->experts % r->groups)
+    return fail(ctx, OSM_EINVAL, "route scores: 1..32 groups that divide the experts");
+  if (r->top_groups == 0 || r->top_groups > r->groups)
+    return fail(ctx, OSM_EINVAL, "route scores: top_groups must be 1..groups");
+  if (r->top_k > r->experts / r->groups * r->top_groups)
+    return fail(ctx, OSM_EINVAL, "route scores: top_k exceeds the experts of the kept groups");
+  if (r->score > OSM_SCORE_SIGMOID || r->group_score > OSM_GROUP_TOP2)
+    return fail(ctx, OSM_EINVAL, "route scores: unknown score or group score");
+  if (!std::isfinite(r->scale)) return fail(ctx, OSM_EINVAL, "route scores: non-finite scale");
+  if (misaligned(r->balance_bias_dev, 4))
+    return fail(ctx, OSM_EINVAL, "route scores: misaligned balance bias");
+  a->E = (int)r->experts;
+  a->k = (int)r->top_k;
+  a->sigmoid = r->score == OSM_SCORE_SIGMOID;
+  // all groups kept: the groups make no difference
+  a->groups = r->top_groups == r->groups ? 1 : (int)r->groups;
+  a->top_groups = r->top_groups == r->groups ? 1 : (int)r->top_groups;
+  a->pair = r->group_score == OSM_GROUP_TOP2;
+  a->renorm = r->renormalize != 0;
+  a->scale = r->scale;
+  a->bias = r->balance_bias_dev;
+  a->status = ctx->sc.status;
+  return OSM_OK;
+}
+
+}  // namespace
+
+int osm_route_scores(osm_context* ctx, const osm_routing* routing, const void* logits, uint32_t type,
+                     uint64_t row_stride, uint32_t tokens, uint32_t* ids, float* weights, float* mass) {
+  if (!ctx) return OSM_EINVAL;
+  osm::RouteArgs a{};
+  if (int rc = routing_args(ctx, routing, &a)) return rc;
+  if (type > OSM_TYPE_F16) return fail(ctx, OSM_EINVAL, "route scores: unknown logits type");
+  if (!logits || !ids || !weights) return fail(ctx, OSM_EINVAL, "route scores: null argument");
+  if (misaligned(logits, type_bytes(type)) || misaligned(ids, 4) || misaligned(weights, 4) || misaligned(mass, 4))
+    return fail(ctx, OSM_EINVAL, "route scores: misaligned argument");
+  if (tokens == 0) return fail(ctx, OSM_EINVAL, "route scores: token count must be non-zero");
+  if (row_stride == 0) row_stride = (uint64_t)a.E;
+  if (row_stride < (uint64_t)a.E || row_stride > (1ull << 40))
+    return fail(ctx, OSM_EINVAL, "route scores: row stride below the number of experts");
+  a.logits = logits;
+  a.type = (int)type;
+  a.row_stride = row_stride;
+  a.tokens = tokens;
+  a.ids = ids;
+  a.weights = weights;
+  a.mass = mass;
+  DeviceGuard dg(ctx->device);
+  Prof p(ctx, kKRouterSelect);
+  const cudaError_t e = osm::launch_route_scores(a, ctx->stream, &ctx->launches);
+  return e == cudaSuccess ? OSM_OK : cuda_fail(ctx, e, "route scores");
+}
+
+int osm_q4_gemv_lora(osm_context* ctx, const uint32_t* packed, const uint16_t* sc, const uint16_t* bi,
+                     uint32_t out_dim, uint32_t in_dim, uint32_t group, const void* x, uint32_t type,
+                     uint64_t x_stride, uint32_t tokens, const osm_lora* lora, const int32_t* adapter,
+                     void* y, uint64_t y_stride) {
+  if (!ctx) return OSM_EINVAL;
+  if (int rc = check_q4(ctx, "q4 gemv lora", packed, sc, bi, out_dim, in_dim, group)) return rc;
+  if (group != 64 || in_dim % 64) return fail(ctx, OSM_EINVAL, "q4 gemv lora: group must be 64");
+  if (in_dim > (1u << 20) || out_dim > (1u << 20))
+    return fail(ctx, OSM_EINVAL, "q4 gemv lora: dimensions up to 2^20");
+  if (type > OSM_TYPE_F16) return fail(ctx, OSM_EINVAL, "q4 gemv lora: unknown type");
+  if (!x || !y || tokens == 0) return fail(ctx, OSM_EINVAL, "q4 gemv lora: null vector or no tokens");
+  if (tokens > (1u << 24)) return fail(ctx, OSM_EINVAL, "q4 gemv lora: at most 2^24 tokens");
+  if (!lora != !adapter)
+    return fail(ctx, OSM_EINVAL, "q4 gemv lora: the adapter table and the tokens' indices go together");
+  if (x_stride == 0) x_stride = in_dim;
+  if (y_stride == 0) y_stride = out_dim;
+  const uint64_t lim = 1ull << 40;
+  if (x_stride < in_dim || y_stride < out_dim || x_stride > lim || y_stride > lim)
+    return fail(ctx, OSM_EINVAL, "q4 gemv lora: row stride below the row's length");
+  const size_t ts = type_bytes(type);
+  if (misaligned(packed, 4) || misaligned(sc, 2) || misaligned(bi, 2) || misaligned(x, ts) || misaligned(y, ts) ||
+      misaligned(adapter, 4))
+    return fail(ctx, OSM_EINVAL, "q4 gemv lora: misaligned argument");
+  {
+    const uintptr_t xa = reinterpret_cast<uintptr_t>(x), ya = reinterpret_cast<uintptr_t>(y);
+    const uint64_t xn = ((uint64_t)(tokens - 1) * x_stride + in_dim) * ts;
+    const uint64_t yn = ((uint64_t)(tokens - 1) * y_stride + out_dim) * ts;
+    if (xa < ya + yn && ya < xa + xn) return fail(ctx, OSM_EINVAL, "q4 gemv lora: x and y overlap");
+  }
+  osm::LoraArgs a{};
+  a.packed = packed;
+  a.scales = sc;
+  a.biases = bi;
+  a.N = (int)out_dim;
+  a.K = (int)in_dim;
+  a.x = x;
+  a.x_type = (int)type;
+  a.x_stride = x_stride;
+  a.tokens = tokens;
+  a.y = y;
+  a.y_stride = y_stride;
+  a.status = ctx->sc.status;
+  if (lora) {
+    if (lora->count == 0 || lora->count > (1u << 24) || lora->rank == 0 || lora->rank > 128)
+      return fail(ctx, OSM_EINVAL, "q4 gemv lora: at least one adapter, rank 1..128");
+    if (lora->type != OSM_TYPE_BF16 && lora->type != OSM_TYPE_F16)
+      return fail(ctx, OSM_EINVAL, "q4 gemv lora: adapters are bf16 or fp16");
+    if (!lora->a_dev || !lora->b_dev) return fail(ctx, OSM_EINVAL, "q4 gemv lora: null adapter table");
+    if (misaligned(lora->a_dev, 2) || misaligned(lora->b_dev, 2) || misaligned(lora->gain_dev, 4) ||
+        misaligned(lora->ranks_dev, 4))
+      return fail(ctx, OSM_EINVAL, "q4 gemv lora: misaligned adapter table");
+    const uint64_t an = (uint64_t)lora->rank * in_dim, bn = (uint64_t)lora->rank * out_dim;
+    a.a_stride = lora->a_stride ? lora->a_stride : an;
+    a.b_stride = lora->b_stride ? lora->b_stride : bn;
+    if (a.a_stride < an || a.b_stride < bn || a.a_stride > lim || a.b_stride > lim)
+      return fail(ctx, OSM_EINVAL, "q4 gemv lora: adapter stride below an adapter's size");
+    a.adapter = adapter;
+    a.a = lora->a_dev;
+    a.b = lora->b_dev;
+    a.a_type = (int)lora->type;
+    a.gain = lora->gain_dev;
+    a.ranks = lora->ranks_dev;
+    a.count = (int)lora->count;
+    a.rank = (int)lora->rank;
+  }
+  DeviceGuard dg(ctx->device);
+  CallWork work(ctx);
+  if (int rc = work.get(osm::lora_workspace(a))) return rc;
+  a.v = static_cast<float*>(work.p);
+  cudaError_t e;
+  {
+    Prof p(ctx, kKOther);
+    e = osm::launch_lora(a, ctx->stream, &ctx->launches);
+  }
+  return work.release(e == cudaSuccess ? OSM_OK : cuda_fail(ctx, e, "q4 gemv lora"));
 }
 
 int osm_swiglu(osm_context* ctx, const float* g, const float* u, float* out, size_t n) {
@@ -1678,6 +1886,39 @@ int osm_moe_route_logits(osm_layer* L, const float* x, uint32_t T, float* logits
   a.pick_ptr = nullptr;
   launch_router_pair(ctx, a);
   return check_launch(ctx, "router");
+}
+
+int osm_moe_route_scores(osm_layer* L, const osm_routing* routing, const float* x, uint32_t T,
+                         uint32_t* ids, float* weights, float* mass) {
+  if (!L || !L->ctx) return OSM_EINVAL;
+  osm_context* ctx = L->ctx;
+  osm::RouteArgs r{};
+  if (int rc = routing_args(ctx, routing, &r)) return rc;
+  if (r.E != L->g.E || r.k != L->g.k)
+    return fail(ctx, OSM_EINVAL, "route scores: experts and top_k must be the layer's");
+  if (!x || !ids || !weights) return fail(ctx, OSM_EINVAL, "route scores: null argument");
+  if (misaligned(x, 4) || misaligned(ids, 4) || misaligned(weights, 4) || misaligned(mass, 4))
+    return fail(ctx, OSM_EINVAL, "route scores: misaligned argument");
+  DeviceGuard dg(ctx->device);
+  if (int rc = layer_ready(L, T, false)) return rc;
+  if (int e = router_x_ok(L, x)) return e;
+  osm::RouterArgs a = router_args(L, x, T);
+  a.exact_logits = 1;
+  {
+    Prof p(ctx, kKRouterLogits);
+    osm::launch_router_logits(a, ctx->stream, &ctx->launches);
+  }
+  if (int rc = check_launch(ctx, "router")) return rc;
+  r.logits = ctx->sc.logits;
+  r.type = (int)OSM_TYPE_F32;
+  r.row_stride = (size_t)L->g.E;
+  r.tokens = T;
+  r.ids = ids;
+  r.weights = weights;
+  r.mass = mass;
+  Prof p(ctx, kKRouterSelect);
+  const cudaError_t e = osm::launch_route_scores(r, ctx->stream, &ctx->launches);
+  return e == cudaSuccess ? OSM_OK : cuda_fail(ctx, e, "route scores");
 }
 
 int osm_moe_forward(osm_layer* L, const float* x, uint32_t T, float* out, uint32_t* ids, float* w,

@@ -41,6 +41,7 @@ struct RouterArgs {
   int B;
   int norm;                 // norm_topk_prob
   int force_exact;
+  int exact_logits;         // logits by the reference's arithmetic for 1-2 tokens too
   int skip_route;           // routing given (osm_moe_experts): gate, fragments, grouping only
   float* logits;            // scratch [B][E]
   float* bounds;            // scratch [B][E]
@@ -429,5 +430,51 @@ cudaError_t launch_host_copy(void* dst, const void* src, size_t bytes, bool afte
 cudaError_t launch_setup_single(int T, const uint8_t* ptr, int* n_active, ActEntry* act, int* n_tg,
                          int* tg_expert, int* tg_begin, int* pair_tok, int* pair_pick,
                          int* out_row, cudaStream_t s, uint64_t* launches);
+
+// The choice of experts from logits (osm_route.cu).  Types: 0 fp32, 1 bf16, 2 fp16.
+struct RouteArgs {
+  const void* logits;       // [tokens] rows of E, row_stride elements apart
+  int type;
+  size_t row_stride;
+  long long tokens;
+  int E, k;
+  int sigmoid;              // sigmoid scores (else softmax)
+  int groups, top_groups;   // groups 1: no groups
+  int pair;                 // value of a group: sum of its two best (else its best)
+  int renorm;
+  float scale;
+  const float* bias;        // [E] or null
+  uint32_t* ids;            // [tokens][k]
+  float* weights;           // [tokens][k]
+  float* mass;              // [tokens] or null
+  uint32_t* status;
+};
+cudaError_t launch_route_scores(const RouteArgs& a, cudaStream_t s, uint64_t* launches);
+
+// A Q4 projection beside per-token low-rank adapters (osm_lora.cu).
+struct LoraArgs {
+  const uint32_t* packed;   // [N][K / 8]
+  const uint16_t* scales;   // [N][K / 64] bf16
+  const uint16_t* biases;
+  int N, K;                 // output and input dimension
+  const void* x;            // [tokens] rows of K
+  int x_type;               // of x and y: 0 fp32, 1 bf16, 2 fp16
+  size_t x_stride;
+  long long tokens;
+  void* y;                  // [tokens] rows of N
+  size_t y_stride;
+  const int* adapter;       // [tokens], negative: none; null: no adapters at all
+  const void* a;            // [count] of [rank][K], a_stride elements apart
+  const void* b;            // [count] of [N][rank]
+  int a_type;               // of a and b: 1 bf16, 2 fp16
+  size_t a_stride, b_stride;
+  const float* gain;        // [count] or null
+  const uint32_t* ranks;    // [count] or null
+  int count, rank;
+  float* v;                 // workspace [tokens][rank]
+  uint32_t* status;
+};
+size_t lora_workspace(const LoraArgs& a);
+cudaError_t launch_lora(const LoraArgs& a, cudaStream_t s, uint64_t* launches);
 
 }  // namespace osm

@@ -1473,10 +1473,10 @@ void launch_exact(const RouterArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-// 1-2 tokens: certified fast logits (the selection checks their bounds);
-// 3+ tokens: exact logits, one thread per (expert, token group).
+// 1-2 tokens: certified fast logits (the selection checks their bounds),
+// unless the caller wants the exact ones; 3+ tokens: exact logits, one thread per (expert, token group).
 void launch_router_logits(const RouterArgs& a, cudaStream_t s, uint64_t* launches) {
-  if (a.B <= 2) {
+  if (a.B <= 2 && !a.exact_logits) {
     launch_logits_t<1, 1>(a, s);
   } else if (a.g.q8) {
     launch_exact2<2>(a, s);  // the layer guarantees H % 128, E % 32 and an aligned x

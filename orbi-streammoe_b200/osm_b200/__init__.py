@@ -32,6 +32,99 @@ def _ptr(t):
     return C.c_void_p(t.data_ptr())
 
 
+_TYPES = {"torch.float32": _lib.OSM_TYPE_F32, "torch.bfloat16": _lib.OSM_TYPE_BF16,
+          "torch.float16": _lib.OSM_TYPE_F16}
+
+
+def _rows(t, length: int, count: int, device: int, what: str):
+    """(type code, row stride) of a CUDA tensor of `count` rows or more of
+    `length` values, each row contiguous."""
+    code = _TYPES.get(str(t.dtype))
+    if code is None:
+        raise ValueError(f"{what}: fp32, bf16 or fp16 rows")
+    if t.dim() != 2 or t.shape[1] != length or t.shape[0] < count:
+        raise ValueError(f"{what}: {count} rows of {length} values expected, got {tuple(t.shape)}")
+    if (length > 1 and t.stride(1) != 1) or (count > 1 and t.stride(0) < length):
+        raise ValueError(f"{what}: rows must be contiguous and must not overlap")
+    if t.device.type != "cuda" or t.device.index != device:
+        raise ValueError(f"{what}: not on the context's device")
+    return code, t.stride(0) if count > 1 else 0
+
+
+def _flat(t, dtype: str, count: int, device: int, what: str):
+    """A contiguous CUDA tensor of `count` values or more of one type."""
+    if t is None:
+        return
+    if str(t.dtype) not in dtype or t.numel() < count or not t.is_contiguous():
+        raise ValueError(f"{what}: {count} contiguous values of {dtype} expected")
+    if t.device.type != "cuda" or t.device.index != device:
+        raise ValueError(f"{what}: not on the context's device")
+
+
+class Routing:
+    """How experts are chosen from router logits (osm_routing): softmax or
+    sigmoid scores, a bias on the choice alone, groups, top-k, renormalised
+    and scaled weights.  Keeps the bias tensor (fp32, on the GPU) alive."""
+
+    def __init__(self, experts: int, top_k: int, score: str = "softmax", bias=None, groups: int = 1,
+                 top_groups: int | None = None, group_score: str = "max", renormalize: bool = True,
+                 scale: float = 1.0):
+        scores = {"softmax": _lib.OSM_SCORE_SOFTMAX, "sigmoid": _lib.OSM_SCORE_SIGMOID}
+        values = {"max": _lib.OSM_GROUP_MAX, "top2": _lib.OSM_GROUP_TOP2}
+        if score not in scores or group_score not in values:
+            raise ValueError("score is softmax or sigmoid, group_score max or top2")
+        if bias is not None:
+            _flat(bias, "torch.float32", experts, bias.device.index, "routing bias")
+        self.bias = bias
+        self.experts, self.top_k = experts, top_k
+        d = self.desc = _lib.RoutingDesc()
+        d.experts, d.top_k, d.score = experts, top_k, scores[score]
+        d.groups, d.top_groups = groups, groups if top_groups is None else top_groups
+        d.group_score, d.renormalize, d.scale = values[group_score], int(bool(renormalize)), scale
+        d.balance_bias_dev = bias.data_ptr() if bias is not None else None
+        self.ref = C.byref(d)
+
+    def _check(self, tokens, ids, weights, mass, device):
+        n = tokens * self.top_k
+        _flat(ids, "torch.int32 torch.uint32", n, device, "route ids")
+        _flat(weights, "torch.float32", n, device, "route weights")
+        _flat(mass, "torch.float32", tokens, device, "route mass")
+        if self.bias is not None and self.bias.device.index != device:
+            raise ValueError("routing bias: not on the context's device")
+
+
+class Lora:
+    """A table of low-rank adapters on the GPU (osm_lora): a [n][rank][in],
+    b [n][out][rank] in bf16 or fp16, each adapter contiguous; gain [n] fp32
+    and ranks [n] int32 (rows of each adapter that count), both optional.
+    Keeps the tensors alive."""
+
+    def __init__(self, a, b, scale=None, ranks=None):
+        n, rank, cin = a.shape
+        cout = b.shape[1]
+        if str(a.dtype) not in ("torch.bfloat16", "torch.float16") or b.dtype != a.dtype:
+            raise ValueError("adapters are bf16 or fp16, A and B alike")
+        if tuple(b.shape) != (n, cout, rank):
+            raise ValueError("A is [n][rank][in], B [n][out][rank]")
+        if not a[0].is_contiguous() or not b[0].is_contiguous():
+            raise ValueError("each adapter must be contiguous")
+        if n > 1 and (a.stride(0) < rank * cin or b.stride(0) < rank * cout):
+            raise ValueError("adapters must not overlap")
+        if a.device.type != "cuda" or b.device != a.device:
+            raise ValueError("adapters must be on one GPU")
+        _flat(scale, "torch.float32", n, a.device.index, "adapter scale")
+        _flat(ranks, "torch.int32 torch.uint32", n, a.device.index, "adapter ranks")
+        self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
+        self.in_dim, self.out_dim, self.device = cin, cout, a.device.index
+        d = self.desc = _lib.LoraDesc()
+        d.count, d.rank, d.type = n, rank, _TYPES[str(a.dtype)]
+        d.a_dev, d.b_dev = a.data_ptr(), b.data_ptr()
+        d.a_stride, d.b_stride = (a.stride(0), b.stride(0)) if n > 1 else (0, 0)
+        d.gain_dev = scale.data_ptr() if scale is not None else None
+        d.ranks_dev = ranks.data_ptr() if ranks is not None else None
+        self.ref = C.byref(d)
+
+
 def expert_layout(hidden: int, inter: int, group: int = 64) -> ExpertLayout:
     L = ExpertLayout()
     rc = lib().osm_expert_layout_packed(hidden, inter, group, C.byref(L))
@@ -123,6 +216,38 @@ class Context:
         self.check(lib().osm_q4_gemv_f32(self.h, _ptr(packed), _ptr(scales), _ptr(biases),
                                          out_dim, in_dim, group, _ptr(x), tokens, _ptr(y)),
                    "q4_gemv_f32")
+
+    def q4_gemv_lora(self, packed, scales_bf16, biases_bf16, out_dim, in_dim, x, tokens, y,
+                     lora: "Lora | None" = None, adapter=None):
+        """y[t] = W x[t] + scale[a] B_a (A_a x[t]) for the adapter a = adapter[t]
+        (int32, negative: none) of the table `lora`; x and y rows of one type
+        (fp32, bf16 or fp16), which may be strided."""
+        code, xs = _rows(x, in_dim, tokens, self.device, "q4_gemv_lora x")
+        ycode, ys = _rows(y, out_dim, tokens, self.device, "q4_gemv_lora y")
+        if ycode != code:
+            raise ValueError("q4_gemv_lora: x and y are of one type")
+        if lora is not None:
+            if lora.in_dim != in_dim or lora.out_dim != out_dim or lora.device != self.device:
+                raise ValueError("q4_gemv_lora: adapters of another projection or device")
+            if adapter is None:
+                raise ValueError("q4_gemv_lora: the tokens' adapter indices are missing")
+            _flat(adapter, "torch.int32", tokens, self.device, "q4_gemv_lora adapter")
+        self.check(lib().osm_q4_gemv_lora(self.h, packed.data_ptr(), scales_bf16.data_ptr(),
+                                          biases_bf16.data_ptr(), out_dim, in_dim, 64, x.data_ptr(), code, xs,
+                                          tokens, lora.ref if lora is not None else None,
+                                          adapter.data_ptr() if adapter is not None else None,
+                                          y.data_ptr(), ys), "q4_gemv_lora")
+
+    def route_scores(self, logits, routing: "Routing", ids, weights, mass=None, tokens=None):
+        """The choice of experts that `routing` describes, from router logits
+        [tokens][experts] (fp32, bf16 or fp16; rows may be strided): ids and
+        weights [tokens][top_k], mass [tokens]."""
+        tokens = logits.shape[0] if tokens is None else tokens
+        code, stride = _rows(logits, routing.experts, tokens, self.device, "route_scores logits")
+        routing._check(tokens, ids, weights, mass, self.device)
+        self.check(lib().osm_route_scores(self.h, routing.ref, logits.data_ptr(), code, stride, tokens,
+                                          ids.data_ptr(), weights.data_ptr(),
+                                          mass.data_ptr() if mass is not None else None), "route_scores")
 
     def swiglu(self, gate, up, out):
         self.check(lib().osm_swiglu(self.h, _ptr(gate), _ptr(up), _ptr(out), gate.numel()), "swiglu")
@@ -272,6 +397,15 @@ class Layer:
         [tokens][experts] fp32."""
         self.ctx.check(lib().osm_moe_route_logits(self.h, _ptr(x), tokens, _ptr(logits), _ptr(ids),
                                                   _ptr(weights), _ptr(mass)), "route_logits")
+
+    def route_scores(self, x, tokens, routing: "Routing", ids, weights, mass=None):
+        """Context.route_scores on this layer's router logits for rows of x
+        (fp32); ids and weights are what run_experts takes."""
+        dev = self.ctx.device
+        _flat(x, "torch.float32", tokens * self.hidden, dev, "route_scores x")
+        routing._check(tokens, ids, weights, mass, dev)
+        self.ctx.check(lib().osm_moe_route_scores(self.h, routing.ref, _ptr(x), tokens, _ptr(ids),
+                                                  _ptr(weights), _ptr(mass)), "route_scores")
 
     def run_qwen_sparse_moe(self, x, tokens, out, ids=None, weights=None, mass=None,
                             shared_gate=None, residual=None, exact_route=False, prefill=False,

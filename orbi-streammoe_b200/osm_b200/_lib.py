@@ -29,12 +29,22 @@ OSM_CACHED_EARLY = 0x80
 OSM_PLAN_SUBLAYER = 0x100
 OSM_PLAN_PROFILE = 0x200
 
+OSM_TYPE_F32 = 0
+OSM_TYPE_BF16 = 1
+OSM_TYPE_F16 = 2
+
+OSM_SCORE_SOFTMAX = 0
+OSM_SCORE_SIGMOID = 1
+OSM_GROUP_MAX = 0
+OSM_GROUP_TOP2 = 1
+
 KERNEL_KINDS = 8
 
 STATUS_NONFINITE = 1
 STATUS_BADMASS = 2
 STATUS_NOTRESIDENT = 4
 STATUS_BADSLOT = 8
+STATUS_BADADAPTER = 256
 
 
 class ExpertLayout(C.Structure):
@@ -53,6 +63,20 @@ class LayerDesc(C.Structure):
                 ("shared_slot_host", C.c_void_p), ("shared_layout", ExpertLayout),
                 ("shared_gate_host", C.c_void_p), ("norm_weight_host", C.c_void_p),
                 ("norm_eps", C.c_float)]
+
+
+class LoraDesc(C.Structure):
+    _fields_ = [("count", C.c_uint32), ("rank", C.c_uint32), ("type", C.c_uint32),
+                ("reserved", C.c_uint32), ("a_dev", C.c_void_p), ("b_dev", C.c_void_p),
+                ("a_stride", C.c_uint64), ("b_stride", C.c_uint64), ("gain_dev", C.c_void_p),
+                ("ranks_dev", C.c_void_p)]
+
+
+class RoutingDesc(C.Structure):
+    _fields_ = [("experts", C.c_uint32), ("top_k", C.c_uint32), ("score", C.c_uint32),
+                ("groups", C.c_uint32), ("top_groups", C.c_uint32), ("group_score", C.c_uint32),
+                ("renormalize", C.c_uint32), ("scale", C.c_float),
+                ("balance_bias_dev", C.c_void_p)]
 
 
 class CacheCounts(C.Structure):
@@ -102,6 +126,11 @@ _SIGS = {
     "osm_ep_forward": (C.c_int, [_P, _P, _P, _P, C.c_uint32, _P, _P, _P, C.c_uint32]),
     "osm_q4_dequant_f32": (C.c_int, [_P, _P, _P, _P, C.c_uint32, C.c_uint32, C.c_uint32, _P]),
     "osm_q4_gemv_f32": (C.c_int, [_P, _P, _P, _P, C.c_uint32, C.c_uint32, C.c_uint32, _P, C.c_uint32, _P]),
+    "osm_q4_gemv_lora": (C.c_int, [_P, _P, _P, _P, C.c_uint32, C.c_uint32, C.c_uint32, _P, C.c_uint32,
+                                   C.c_uint64, C.c_uint32, C.POINTER(LoraDesc), _P, _P, C.c_uint64]),
+    "osm_route_scores": (C.c_int, [_P, C.POINTER(RoutingDesc), _P, C.c_uint32, C.c_uint64, C.c_uint32,
+                                   _P, _P, _P]),
+    "osm_moe_route_scores": (C.c_int, [_P, C.POINTER(RoutingDesc), _P, C.c_uint32, _P, _P, _P]),
     "osm_swiglu": (C.c_int, [_P, _P, _P, _P, C.c_size_t]),
     "osm_weighted_accumulate": (C.c_int, [_P, _P, C.c_float, _P, C.c_size_t]),
     "osm_rms_norm": (C.c_int, [_P, _P, C.c_uint32, C.c_uint32, _P, C.c_float, C.c_uint32]),
