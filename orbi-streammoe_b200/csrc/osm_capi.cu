@@ -1067,6 +1067,7 @@ int osm_context_create(int device, uint32_t max_tokens, osm_context** out) {
   osm::init_prefill_attributes(ctx->max_smem);
   osm::init_tc_attributes(ctx->max_smem);
   osm::init_dg_attributes(ctx->max_smem);
+  osm::init_lora_attributes(ctx->max_smem);
   {
     const char* v = std::getenv("OSM_DISABLE_TC");
     ctx->tc_enabled = !(v && v[0] && v[0] != '0');
@@ -1486,12 +1487,11 @@ int osm_q4_gemv_lora(osm_context* ctx, const uint32_t* packed, const uint16_t* s
   }
   DeviceGuard dg(ctx->device);
   CallWork work(ctx);
-  if (int rc = work.get(osm::lora_workspace(a))) return rc;
-  a.v = static_cast<float*>(work.p);
+  if (int rc = work.get(osm::lora_workspace(a, ctx->num_sms))) return rc;
   cudaError_t e;
   {
     Prof p(ctx, kKOther);
-    e = osm::launch_lora(a, ctx->stream, &ctx->launches);
+    e = osm::launch_lora(a, work.p, ctx->num_sms, ctx->stream, &ctx->launches);
   }
   return work.release(e == cudaSuccess ? OSM_OK : cuda_fail(ctx, e, "q4 gemv lora"));
 }

@@ -471,10 +471,17 @@ struct LoraArgs {
   const float* gain;        // [count] or null
   const uint32_t* ranks;    // [count] or null
   int count, rank;
-  float* v;                 // workspace [tokens][rank]
   uint32_t* status;
+  // filled by launch_lora: workspace, shape of a launch, alignments
+  unsigned char* planes;    // x as matrix operands [tile][K / 64][plane][NT][128 bytes]
+  int* ex;                  // [tokens] exponent of each row
+  float* v;                 // [tokens] rows of v_stride: gain A x
+  size_t v_stride;
+  int NT, split;            // tokens per tile, CTAs per tile
+  int x_vec, w_vec, a_vec, b_vec;  // 16-byte aligned rows
 };
-size_t lora_workspace(const LoraArgs& a);
-cudaError_t launch_lora(const LoraArgs& a, cudaStream_t s, uint64_t* launches);
+cudaError_t init_lora_attributes(int max_smem);
+size_t lora_workspace(const LoraArgs& a, int sms);
+cudaError_t launch_lora(const LoraArgs& a, void* workspace, int sms, cudaStream_t s, uint64_t* launches);
 
 }  // namespace osm
