@@ -475,10 +475,16 @@ struct LoraArgs {
   // filled by launch_lora: workspace, shape of a launch, alignments
   unsigned char* planes;    // x as matrix operands [tile][K / 64][plane][NT][128 bytes]
   int* ex;                  // [tokens] exponent of each row
-  float* v;                 // [tokens] rows of v_stride: gain A x
+  int* ew;                  // [N] of each row of W
+  uint32_t* wbias;          // biases as operands [N / 128][stage][32][128]
+  float* v;                 // gain A x: [tokens][v_stride], or bf16 [tokens][v_planes][v_stride]
   size_t v_stride;
+  int v_planes;             // 0: fp32
   int NT, split;            // tokens per tile, CTAs per tile
-  int x_vec, w_vec, a_vec, b_vec;  // 16-byte aligned rows
+  // the prep kernel: blocks for v (tiles of v_tile tokens, v_slots blocks per
+  // tile for its adapters), for W, and threads per row of x
+  int v_blocks, v_tile, v_slots, w_blocks, row_threads;
+  int x_vec, w_vec, m_vec, a_vec, b_vec;  // 16-byte aligned rows (m: scales and biases)
 };
 cudaError_t init_lora_attributes(int max_smem);
 size_t lora_workspace(const LoraArgs& a, int sms);

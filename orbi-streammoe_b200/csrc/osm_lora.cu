@@ -7,26 +7,30 @@
 //
 // Two kernels, whatever the number of tokens.
 //
-// lora_prep_kernel, over tiles of 16 tokens: the rows of x as fp16 operands of
-// the tensor cores, each row scaled by a power of two so that its largest
-// value lies in [2^14, 2^15) (fp32 rows as hi + lo, 22 bits; bf16 and fp16
-// rows exactly), and v[t] = gain A_a x[t] by tf32 matrix products (x as hi +
-// lo for fp32 rows), once for every distinct adapter of a tile.
+// Up to 8 tokens: lora_prep_kernel (v[t] = gain A_a x[t]) and, beside it,
+// lora_decode_kernel (W x on CUDA cores, then B_a v).
 //
-// lora_gemm_kernel: D[128 rows of W][N tokens] on tcgen05.  Weights go from Q4
-// to fp16 (hi + lo for fp32 rows) into tensor memory, scaled by a power of two
-// per row of W in the same way; x comes by bulk copies.  The adapters are
-// further steps of the same sum: for the distinct adapters of the tile, B_a
-// (rows of W) against v with zeros in the tokens of other adapters, in bf16
-// planes, which have the range for any ratio between W, B, x and v.  So a tile
-// of many requests needs no sorting and no second pass over y.
+// More: lora_prep_kernel also writes the rows of x as fp16 operands of the
+// tensor cores, each row scaled by a power of two so that its largest value
+// lies in [2^14, 2^15) (fp32 rows as hi + lo, 22 bits; bf16 and fp16 rows
+// exactly), and the sums of their groups of 64.  lora_gemm_kernel then computes
+// D[128 rows of W][N tokens] on tcgen05.  A weight is scale (q - 8) + (bias + 8
+// scale): the first term is exact in fp16 (8 + 3 bits) and goes to tensor
+// memory, scaled by a power of two per row of W; the second multiplies the
+// group sums in further steps of the same sum.  So are the adapters: for the
+// distinct adapters of the tile, B_a against v with zeros in the tokens of
+// other adapters, in bf16 planes, which have the range for any ratio between
+// W, B, x and v.  A tile of many requests needs no sorting and no second pass
+// over y.
 //
-// What rounds: fp32 rows hold 22 bits of x and w (products to about 2^-22) and
-// sums of 16 products per step; the tensor core's accumulation drops what lies
-// below the accumulator's last place, so after every 4 K groups (16 steps) the
+// v is computed by tf32 matrix products (x as hi + lo for fp32 rows), once for
+// every distinct adapter of a tile of tokens.
+//
+// What rounds: fp32 rows hold 22 bits of x (products to about 2^-22) and sum
+// 16 products per step; the tensor core's accumulation drops what lies below
+// the accumulator's last place, so after every 4 K groups (32 steps) the
 // partial sum leaves tensor memory and is added in registers, which keeps the
-// loss under 1e-6.  16-bit rows round each weight once to fp16 (2^-12, below
-// the rounding of y), v to 16 bits, and y once.
+// loss under 1e-6.  16-bit rows round v to 16 bits and y once.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -96,12 +100,6 @@ __device__ __forceinline__ int row_exponent(float m) {
   return max(e, -100);
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // |e| <= 126
-// v 2^e for any e a product of two rows' exponents can have
-__device__ __forceinline__ float scale_by(float v, int e) {
-  const int h = e >> 1;
-  return v * pow2(h) * pow2(e - h);
-}
-
 // The adapter of token t and its rank; -1 and rank 0 where there is none.  An
 // index past the table counts as none and sets the status bit.
 __device__ __forceinline__ int adapter_of(const LoraArgs& a, long long t, int& rank) {
@@ -116,149 +114,475 @@ __device__ __forceinline__ int adapter_of(const LoraArgs& a, long long t, int& r
   return id;
 }
 
-// ---------------------------------------------------------------- prep
+// ---------------------------------------------------------------- v = gain A x
 
-__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr int kPrepRows = 16;   // tokens per tile of the prep kernel
-constexpr int kPrepWarps = 8;
-constexpr int kPrepCols = 32;   // rank columns per pass
+constexpr int kPrepWarps = 16;
+constexpr int kPrepThreads = kPrepWarps * 32;
+constexpr int kVCols = 32;   // rows of A per pass
 
-// Blocks (tile, 0): operand planes of 16 rows.  Blocks (tile, y > 0): v for the
-// tile's distinct adapters y - 1, y - 1 + (gridDim.y - 1), ...
-template <int XT, int AT>
-__global__ void __launch_bounds__(kPrepWarps * 32) lora_prep_kernel(const LoraArgs a) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long t0 = (long long)blockIdx.x * kPrepRows;
-  pdl_wait();
-  pdl_trigger();
-  constexpr int PB = XT == 0 ? 2 : 1;
-  if (blockIdx.y == 0) {
-    for (int r = warp; r < kPrepRows; r += kPrepWarps) {
-      const long long t = t0 + r;
-      const bool live = t < a.tokens;
-      const size_t row = (size_t)t * a.x_stride;
-      int ex = 0;
-      if (live) {
-        float m = 0.0f;
-        for (int i = lane * 8; i < a.K; i += 256) {
-          float v[8];
-          load8<XT>(a.x, row + i, a.x_vec, v);
+// 8 consecutive values as loaded: two words of four bytes per value pair for
+// fp32, one for 16-bit types
+template <int TYPE>
+struct Raw8 {
+  uint32_t w[TYPE == 0 ? 8 : 4];
+};
+template <int TYPE>
+__device__ __forceinline__ Raw8<TYPE> load_raw8(const void* p, size_t i, bool vec) {
+  Raw8<TYPE> r;
+  if constexpr (TYPE == 0) {
+    float v[8];
+    load8<0>(p, i, vec, v);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
-        }
-        ex = row_exponent(warp_max(m));
-      }
-      if (lane == 0) a.ex[t] = ex;
-      const float sc = pow2(-ex);
-      const int row_in = (int)(t % a.NT);
-      unsigned char* tile = a.planes + (size_t)(t / a.NT) * (a.K >> 6) * PB * a.NT * 128 + (size_t)row_in * 128;
-      for (int i = lane * 8; i < a.K; i += 256) {
-        float v[8] = {};
-        if (live) load8<XT>(a.x, row + i, a.x_vec, v);
-        uint32_t hi[4], lo[4];
+    for (int e = 0; e < 8; ++e) r.w[e] = __float_as_uint(v[e]);
+  } else if (vec) {
+    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    r.w[0] = a.x;
+    r.w[1] = a.y;
+    r.w[2] = a.z;
+    r.w[3] = a.w;
+  } else {
+    const uint16_t* q = static_cast<const uint16_t*>(p) + i;
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const float x0 = v[2 * p] * sc, x1 = v[2 * p + 1] * sc;
-          const __half2 h = __floats2half2_rn(x0, x1);
-          hi[p] = h2u(h);
-          if constexpr (PB == 2) {
-            const float2 f = __half22float2(h);
-            lo[p] = h2u(__floats2half2_rn(x0 - f.x, x1 - f.y));
-          }
-        }
-        unsigned char* at = tile + (size_t)(i >> 6) * PB * a.NT * 128 + ((((i >> 3) & 7) ^ (row_in & 7)) << 4);
-        *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (PB == 2)
-          *reinterpret_cast<uint4*>(at + (size_t)a.NT * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-    }
-    return;
+    for (int e = 0; e < 4; ++e) r.w[e] = pack2(q[2 * e], q[2 * e + 1]);
   }
-  __shared__ int s_id[kPrepRows], s_rank[kPrepRows], s_list[kPrepRows], s_n;
-  __shared__ float s_red[kPrepWarps][kPrepRows][kPrepCols];
+  return r;
+}
+// values 2 s and 2 s + 1
+template <int TYPE>
+__device__ __forceinline__ void raw_pair(const Raw8<TYPE>& r, int s, float& a, float& b) {
+  if constexpr (TYPE == 0) {
+    a = __uint_as_float(r.w[2 * s]);
+    b = __uint_as_float(r.w[2 * s + 1]);
+  } else {
+    unpack2<TYPE>(r.w[s], a, b);
+  }
+}
+
+// One tile of 16 MT tokens: v for the tile's distinct adapters slot, slot +
+// v_slots, ...  MT = 1: 16 warps split K; MT = 2: 8, so that a prompt's tokens
+// share the rows of A twice over.  v goes out in fp32 (few tokens) or as the
+// bf16 planes of the matrix kernel, [token][plane][v_stride].
+template <int XT, int AT, int MT>
+__device__ __forceinline__ void prep_v(const LoraArgs& a, int block, float* red) {
+  constexpr int TOK = 16 * MT, KW = kPrepWarps / MT;
+  __shared__ alignas(16) int s_id[TOK];
+  __shared__ int s_rank[TOK], s_list[TOK], s_n;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int slot = block % a.v_slots;
+  const long long t0 = (long long)(block / a.v_slots) * TOK;
   if (warp == 0) {
     int rank = 0, id = -1;
-    if (lane < kPrepRows && t0 + lane < a.tokens) id = adapter_of(a, t0 + lane, rank);
-    if (lane < kPrepRows) {
+    if (lane < TOK && t0 + lane < a.tokens) id = adapter_of(a, t0 + lane, rank);
+    if (lane < TOK) {
       s_id[lane] = id;
       s_rank[lane] = rank;
     }
     const uint32_t same = __match_any_sync(kAllLanes, id);
-    const bool first = lane < kPrepRows && rank > 0 && (int)(__ffs(same) - 1) == lane;
+    const bool first = lane < TOK && rank > 0 && (int)__ffs(same) - 1 == lane;
     const uint32_t firsts = __ballot_sync(kAllLanes, first);
     if (first) s_list[__popc(firsts & ((1u << lane) - 1u))] = lane;
     if (lane == 0) s_n = __popc(firsts);
   }
   __syncthreads();
-  const int g = lane >> 2, q = lane & 3;
-  for (int d = (int)blockIdx.y - 1; d < s_n; d += (int)gridDim.y - 1) {
+  const int g = lane >> 2, q = lane & 3, mi = warp % MT, kw = warp / MT;
+  const int r0 = mi * 16 + g;
+  for (int d = slot; d < s_n; d += a.v_slots) {
     const int id = s_id[s_list[d]], rank = s_rank[s_list[d]];
-    const bool in0 = s_id[g] == id, in1 = s_id[g + 8] == id;
-    const size_t x0 = (size_t)(t0 + g) * a.x_stride, x1 = (size_t)(t0 + g + 8) * a.x_stride;
+    const float gain = a.gain ? a.gain[id] : 1.0f;
+    const bool in0 = s_id[r0] == id, in1 = s_id[r0 + 8] == id;
+    const bool any = __any_sync(kAllLanes, in0 || in1);
+    const size_t x0 = (size_t)(t0 + r0) * a.x_stride, x1 = (size_t)(t0 + r0 + 8) * a.x_stride;
     const size_t arow = (size_t)id * a.a_stride;
-    for (int j0 = 0; j0 < rank; j0 += kPrepCols) {
-      float acc[kPrepCols / 8][4] = {};
+    for (int j0 = 0; j0 < rank; j0 += kVCols) {
+      float acc[kVCols / 8][4] = {};
       // K in steps of 32: the thread's 8 values of a row are the k and k + 4
       // positions of four 8-wide matrix steps (the order of K is free as long
       // as both operands use the same one)
+      if (any) {
 #pragma unroll 2
-      for (int c = warp; c < a.K / 32; c += kPrepWarps) {
-        const int i = c * 32 + q * 8;
-        float xa[8] = {}, xb[8] = {};
-        if (in0) load8<XT>(a.x, x0 + i, a.x_vec, xa);
-        if (in1) load8<XT>(a.x, x1 + i, a.x_vec, xb);
+        for (int c = kw; c < a.K / 32; c += KW) {
+          const int i = c * 32 + q * 8;
+          Raw8<XT> xa{}, xb{};
+          Raw8<AT> w[kVCols / 8] = {};
+          if (in0) xa = load_raw8<XT>(a.x, x0 + i, a.x_vec);
+          if (in1) xb = load_raw8<XT>(a.x, x1 + i, a.x_vec);
 #pragma unroll
-        for (int n = 0; n < kPrepCols / 8; ++n) {
-          const int j = j0 + n * 8 + g;
-          float w[8] = {};
-          if (j0 + n * 8 < rank) {
-            if (j < rank) load8<AT>(a.a, arow + (size_t)j * a.K + i, a.a_vec, w);
+          for (int n = 0; n < kVCols / 8; ++n) {
+            const int j = j0 + n * 8 + g;
+            if (j < rank) w[n] = load_raw8<AT>(a.a, arow + (size_t)j * a.K + i, a.a_vec);
+          }
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-              const uint32_t b0 = __float_as_uint(w[2 * s]), b1 = __float_as_uint(w[2 * s + 1]);
-              uint32_t h[4] = {__float_as_uint(xa[2 * s]), __float_as_uint(xb[2 * s]), __float_as_uint(xa[2 * s + 1]),
-                               __float_as_uint(xb[2 * s + 1])};
+          for (int s = 0; s < 4; ++s) {
+            float f[4];
+            raw_pair<XT>(xa, s, f[0], f[2]);
+            raw_pair<XT>(xb, s, f[1], f[3]);
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              h[e] = __float_as_uint(f[e]);
               if constexpr (XT == 0) {
-                uint32_t l[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float f = __uint_as_float(h[e]);
-                  h[e] &= 0xFFFFE000u;
-                  l[e] = __float_as_uint(f - __uint_as_float(h[e]));
-                }
-                mma_tf32(acc[n], l, b0, b1);
+                h[e] &= 0xFFFFE000u;
+                l[e] = __float_as_uint(f[e] - __uint_as_float(h[e]));
               }
-              mma_tf32(acc[n], h, b0, b1);
+            }
+#pragma unroll
+            for (int n = 0; n < kVCols / 8; ++n) {
+              if (j0 + n * 8 >= rank) continue;
+              float b0, b1;
+              raw_pair<AT>(w[n], s, b0, b1);
+              if constexpr (XT == 0)
+                mma_tf32(acc[n], l[0], l[1], l[2], l[3], __float_as_uint(b0), __float_as_uint(b1));
+              mma_tf32(acc[n], h[0], h[1], h[2], h[3], __float_as_uint(b0), __float_as_uint(b1));
             }
           }
         }
       }
 #pragma unroll
-      for (int n = 0; n < kPrepCols / 8; ++n) {
-        s_red[warp][g][n * 8 + 2 * q] = acc[n][0];
-        s_red[warp][g][n * 8 + 2 * q + 1] = acc[n][1];
-        s_red[warp][g + 8][n * 8 + 2 * q] = acc[n][2];
-        s_red[warp][g + 8][n * 8 + 2 * q + 1] = acc[n][3];
+      for (int n = 0; n < kVCols / 8; ++n) {
+        float* at = red + ((size_t)kw * TOK + r0) * kVCols + n * 8 + 2 * q;
+        *reinterpret_cast<float2*>(at) = make_float2(acc[n][0], acc[n][1]);
+        *reinterpret_cast<float2*>(at + 8 * kVCols) = make_float2(acc[n][2], acc[n][3]);
       }
       __syncthreads();
-      const float gain = a.gain ? a.gain[id] : 1.0f;
-      for (int o = tid; o < kPrepRows * kPrepCols; o += kPrepWarps * 32) {
-        const int r = o / kPrepCols, j = o % kPrepCols;
+      for (int o = tid; o < TOK * kVCols; o += kPrepThreads) {
+        const int r = o / kVCols, j = o % kVCols;
         float s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kPrepWarps; ++w) s += s_red[w][r][j];
-        // whole granules of 16: zeros behind the adapter's rank
-        if (s_id[r] == id && j0 + j < ((rank + 15) & ~15))
-          a.v[(size_t)(t0 + r) * a.v_stride + j0 + j] = j0 + j < rank ? gain * s : 0.0f;
+        for (int w = 0; w < KW; ++w) s += red[((size_t)w * TOK + r) * kVCols + j];
+        // whole pieces of 16: zeros behind the adapter's rank
+        if (s_id[r] == id && j0 + j < ((rank + 15) & ~15)) {
+          s = j0 + j < rank ? gain * s : 0.0f;
+          if (a.v_planes == 0) {
+            a.v[(size_t)(t0 + r) * a.v_stride + j0 + j] = s;
+          } else {
+            uint16_t* at = reinterpret_cast<uint16_t*>(a.v) + (size_t)(t0 + r) * a.v_planes * a.v_stride + j0 + j;
+            for (int p = 0; p < a.v_planes; ++p) {
+              const uint32_t b = pack_bf2(s, 0.0f) & 0xFFFFu;
+              at[(size_t)p * a.v_stride] = (uint16_t)b;
+              s -= bf_lo(b);
+            }
+          }
+        }
       }
       __syncthreads();
     }
   }
+}
+
+// ---------------------------------------------------------------- x as operands
+
+// fp16 planes of one row, TPR threads per row: a warp where there are rows
+// enough to fill the GPU, else a block (one trip to memory for a row of 2048
+// values instead of eight).  A thread keeps its first vectors in registers
+// between the maximum and the conversion.
+template <int XT, int TPR>
+__device__ __forceinline__ void prep_row(const LoraArgs& a, long long t) {
+  constexpr int PB = XT == 0 ? 2 : 1, KEEP = TPR == 32 ? 4 : 1;
+  __shared__ float s_max[kPrepWarps];
+  const int lane = threadIdx.x % TPR;
+  const bool live = t < a.tokens;
+  const size_t row = (size_t)t * a.x_stride;
+  const int row_in = (int)(t % a.NT), nk = a.K >> 6, nkp = nk + (nk + 63) / 64;
+  unsigned char* tile = a.planes + (size_t)(t / a.NT) * nkp * PB * a.NT * 128 + (size_t)row_in * 128;
+  float kept[KEEP][8];
+  float m = 0.0f;
+#pragma unroll
+  for (int c = 0; c < KEEP; ++c) {
+    const int i = (c * TPR + lane) * 8;
+    if (live && i < a.K) {
+      load8<XT>(a.x, row + i, a.x_vec, kept[c]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) kept[c][e] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < KEEP; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(kept[c][e]));
+  if (live) {
+#pragma unroll 4
+    for (int i = (KEEP * TPR + lane) * 8; i < a.K; i += TPR * 8) {
+      float v[8];
+      load8<XT>(a.x, row + i, a.x_vec, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
+    }
+  }
+  m = warp_max(m);
+  if constexpr (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kPrepWarps; ++w) m = fmaxf(m, s_max[w]);
+  }
+  const int ex = row_exponent(m);
+  if (lane == 0) a.ex[t] = ex;
+  const float sc = pow2(-ex);
+  auto chunk_at = [&](int k, int unit) {
+    return tile + (size_t)k * PB * a.NT * 128 + ((unit ^ (row_in & 7)) << 4);
+  };
+  // the 8 values from i on and, by 8 threads together, their group's sum
+  auto put = [&](int i, const float (&v)[8]) {
+    uint32_t hi[4], lo[4];
+    float sum = 0.0f;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const float x0 = v[p] * sc, x1 = v[p + 4] * sc;   // the order of the weights' pairs
+      sum += x0 + x1;
+      const __half2 h = __floats2half2_rn(x0, x1);
+      hi[p] = h2u(h);
+      if constexpr (PB == 2) {
+        const float2 f = __half22float2(h);
+        lo[p] = h2u(__floats2half2_rn(x0 - f.x, x1 - f.y));
+      }
+    }
+    unsigned char* at = chunk_at(i >> 6, (i >> 3) & 7);
+    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if constexpr (PB == 2) *reinterpret_cast<uint4*>(at + (size_t)a.NT * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    // whole groups are in or out, so these 8 lanes are all here
+    const uint32_t mask = 0xFFu << (threadIdx.x & 24);
+    sum += __shfl_xor_sync(mask, sum, 1);
+    sum += __shfl_xor_sync(mask, sum, 2);
+    sum += __shfl_xor_sync(mask, sum, 4);
+    if ((threadIdx.x & 7) == 0) {
+      const int grp = i >> 6, col = grp & 63;
+      const float x = sum * (1.0f / 64.0f);  // stays below 2^15; the biases carry the 64
+      const __half h = __float2half_rn(x);
+      unsigned char* gat = chunk_at(nk + (grp >> 6), col >> 3) + (col & 7) * 2;
+      *reinterpret_cast<__half*>(gat) = h;
+      if constexpr (PB == 2) *reinterpret_cast<__half*>(gat + (size_t)a.NT * 128) = __float2half_rn(x - __half2float(h));
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < KEEP; ++c) {
+    const int i = (c * TPR + lane) * 8;
+    if (i < a.K) put(i, kept[c]);
+  }
+#pragma unroll 4
+  for (int i = (KEEP * TPR + lane) * 8; i < a.K; i += TPR * 8) {
+    float v[8] = {};
+    if (live) load8<XT>(a.x, row + i, a.x_vec, v);
+    put(i, v);
+  }
+  // zeros behind the last group's sum
+  for (int c = nk + lane; c < (nkp - nk) * 64; c += TPR) {
+    unsigned char* at = chunk_at(nk + (c >> 6), (c & 63) >> 3) + (c & 7) * 2;
+    *reinterpret_cast<__half*>(at) = __float2half_rn(0.0f);
+    if constexpr (PB == 2) *reinterpret_cast<__half*>(at + (size_t)a.NT * 128) = __float2half_rn(0.0f);
+  }
+}
+
+__device__ __forceinline__ uint4 load_meta(const LoraArgs& a, const uint16_t* base, int o, int k8);
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i);
+
+// The exponents of 128 rows of W and their biases as operands.  A weight is
+// scale (q - 8) + c with c = bias + 8 scale; the exponent is that of the largest
+// of 16 |scale|, which keeps the converters' 24 scale in range, and 64 |c| (the
+// groups' sums of x are kept as 1/64, so c carries the 64).  Operands [stage][pair of groups][row]: fp16 pairs, hi, and for fp32
+// rows of x lo in a stage of its own.  Four threads per row.
+template <bool F32>
+__device__ __forceinline__ void prep_weights(const LoraArgs& a, int tile) {
+  constexpr int PARTS = kPrepThreads / 128;
+  const int row = threadIdx.x / PARTS, part = threadIdx.x % PARTS, o = tile * 128 + row;
+  const int nk = a.K >> 6, n8 = (nk + 7) / 8, nbk = (nk + 63) / 64;
+  auto mid = [](float s, float b) { return 64.0f * fmaf(8.0f, s, b); };
+  float m = 0.0f;
+  if (o < a.N) {
+#pragma unroll 4
+    for (int k8 = part; k8 < n8; k8 += PARTS) {
+      const uint4 sv = load_meta(a, a.scales, o, k8), bv = load_meta(a, a.biases, o, k8);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const uint32_t sw = word_of(sv, p), bw = word_of(bv, p);
+        m = fmaxf(m, fmaxf(16.0f * fabsf(bf_lo(sw)), fabsf(mid(bf_lo(sw), bf_lo(bw)))));
+        m = fmaxf(m, fmaxf(16.0f * fabsf(bf_hi(sw)), fabsf(mid(bf_hi(sw), bf_hi(bw)))));
+      }
+    }
+  }
+  m = fmaxf(m, __shfl_xor_sync(kAllLanes, m, 1));
+  m = fmaxf(m, __shfl_xor_sync(kAllLanes, m, 2));
+  const int ew = row_exponent(m);
+  if (part == 0) a.ew[o] = ew;
+  const float sc = pow2(-ew);
+  uint32_t* out = a.wbias + (size_t)tile * (F32 ? 2 : 1) * nbk * 32 * 128 + row;
+#pragma unroll 4
+  for (int k8 = part; k8 < nbk * 8; k8 += PARTS) {
+    uint4 sv = make_uint4(0, 0, 0, 0), bv = sv;
+    if (o < a.N && k8 < n8) {
+      sv = load_meta(a, a.scales, o, k8);
+      bv = load_meta(a, a.biases, o, k8);
+    }
+    const int bi = k8 >> 3, col = (k8 & 7) * 4;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const uint32_t sw = word_of(sv, p), bw = word_of(bv, p);
+      const float f0 = mid(bf_lo(sw), bf_lo(bw)) * sc, f1 = mid(bf_hi(sw), bf_hi(bw)) * sc;
+      const __half2 h = __floats2half2_rn(f0, f1);
+      if constexpr (F32) {
+        const float2 f = __half22float2(h);
+        out[(size_t)((bi * 2) * 32 + col + p) * 128] = h2u(h);
+        out[(size_t)((bi * 2 + 1) * 32 + col + p) * 128] = h2u(__floats2half2_rn(f0 - f.x, f1 - f.y));
+      } else {
+        out[(size_t)(bi * 32 + col + p) * 128] = h2u(h);
+      }
+    }
+  }
+}
+
+// First the blocks for v, then those for W, then rows of x, up to the next
+// multiple of 16 (zero rows behind the last).
+template <int XT, int AT>
+__global__ void __launch_bounds__(kPrepThreads, 2) lora_prep_kernel(const __grid_constant__ LoraArgs a) {
+  __shared__ alignas(16) float s_red[kPrepWarps * 16 * kVCols];
+  pdl_wait();
+  pdl_trigger();
+  if ((int)blockIdx.x < a.v_blocks) {
+    if (a.v_tile == 16) prep_v<XT, AT, 1>(a, (int)blockIdx.x, s_red);
+    else prep_v<XT, AT, 2>(a, (int)blockIdx.x, s_red);
+    return;
+  }
+  if ((int)blockIdx.x < a.v_blocks + a.w_blocks) {
+    prep_weights<XT == 0>(a, (int)blockIdx.x - a.v_blocks);
+    return;
+  }
+  const long long b = (long long)blockIdx.x - a.v_blocks - a.w_blocks;
+  if (a.row_threads == kPrepThreads) {
+    prep_row<XT, kPrepThreads>(a, b);
+  } else {
+    const long long t = b * kPrepWarps + (threadIdx.x >> 5);
+    if (t < (a.tokens + 15) / 16 * 16) prep_row<XT, 32>(a, t);
+  }
+}
+
+// ---------------------------------------------------------------- few tokens
+
+// Up to 8 tokens: the projection on CUDA cores in fp32, one warp per ROWS rows
+// of W and all tokens, lane l the groups l, l + 32, ... of a row.  Bound by
+// latency: a launch reads about 2.4 MB for 2048 x 2048.  It starts beside the
+// kernel that computes v and waits for it only before the adapters' term.
+// x is kept in shared memory in fp32; 16-byte piece c of group g sits at piece
+// c ^ (g & 15), so that the lanes of a warp, which read the same piece of 32
+// groups, meet all banks.
+constexpr int kDecWarps = 8;
+constexpr int kDecTokens = 8;
+constexpr size_t kDecSmem = 128 << 10;   // x in shared memory, most
+
+template <int XT, int AT, int TT, int ROWS>
+__global__ void __launch_bounds__(kDecWarps * 32) lora_decode_kernel(const __grid_constant__ LoraArgs a) {
+  extern __shared__ float4 dec_x[];   // [token][K / 4]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = a.K >> 6, T = (int)a.tokens;
+  const int o0 = ((int)blockIdx.x * kDecWarps + warp) * ROWS;
+  // without a kernel for v before it this one may start early itself
+  if (!a.adapter) pdl_wait();
+  for (int i = tid; i < T * G * 8; i += kDecWarps * 32) {
+    const int t = i / (G * 8), p = i - t * (G * 8);   // 8 values from 8 p on
+    float v[8];
+    load8<XT>(a.x, (size_t)t * a.x_stride + p * 8, a.x_vec, v);
+    const int g = p >> 3, c = (p & 7) * 2;
+    float4* row = dec_x + ((size_t)t * G + g) * 16;
+    row[c ^ (g & 15)] = make_float4(v[0], v[1], v[2], v[3]);
+    row[(c + 1) ^ (g & 15)] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+  float acc[ROWS][TT];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[r][t] = 0.0f;
+  uint4 w[ROWS][2];
+  float sc[ROWS], bi[ROWS];
+  auto load_w = [&](int g) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const int o = min(o0 + r, a.N - 1);
+      const uint32_t* p = a.packed + (size_t)o * (a.K >> 3) + g * 8;
+      if (a.w_vec) {
+        w[r][0] = __ldg(reinterpret_cast<const uint4*>(p));
+        w[r][1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+      } else {
+        w[r][0] = make_uint4(p[0], p[1], p[2], p[3]);
+        w[r][1] = make_uint4(p[4], p[5], p[6], p[7]);
+      }
+      sc[r] = bf16_bits_to_f32(a.scales[(size_t)o * G + g]);
+      bi[r] = bf16_bits_to_f32(a.biases[(size_t)o * G + g]);
+    }
+  };
+  if (o0 < a.N && lane < G) load_w(lane);
+  __syncthreads();
+  if (o0 >= a.N) return;
+  for (int g = lane; g < G; g += 32) {
+    if (g >= 32) load_w(g);
+    const float4* xg = dec_x + (size_t)g * 16;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      float wf[ROWS][4];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const uint4 v = w[r][c >> 3];
+        const uint32_t word = (c >> 1 & 3) == 0 ? v.x : (c >> 1 & 3) == 1 ? v.y : (c >> 1 & 3) == 2 ? v.z : v.w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // 2^23 + q, exactly q after the subtraction
+          const float f = __uint_as_float(((word >> (16 * (c & 1) + 4 * e)) & 15u) | 0x4B000000u) - 8388608.0f;
+          wf[r][e] = fmaf(sc[r], f, bi[r]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        if (t < T) {
+          const float4 x = xg[(size_t)t * G * 16 + (c ^ (g & 15))];
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r)
+            acc[r][t] = fmaf(wf[r][3], x.w, fmaf(wf[r][2], x.z, fmaf(wf[r][1], x.y, fmaf(wf[r][0], x.x, acc[r][t]))));
+        }
+      }
+    }
+  }
+  if (a.adapter) {
+    int id[TT], rank[TT];
+    float b[ROWS][TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      id[t] = -1;
+      rank[t] = 0;
+      if (t < T) id[t] = adapter_of(a, t, rank[t]);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+        b[r][t] = lane < rank[t] && o0 + r < a.N
+                      ? load_val<AT>(a.b, (size_t)id[t] * a.b_stride + (size_t)(o0 + r) * a.rank + lane) : 0.0f;
+    }
+    pdl_wait();  // v is complete from here on
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      for (int j = lane; j < rank[t]; j += 32) {
+        const float v = a.v[(size_t)t * a.v_stride + j];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          const float bv = j == lane ? b[r][t]
+                           : o0 + r < a.N
+                               ? load_val<AT>(a.b, (size_t)id[t] * a.b_stride + (size_t)(o0 + r) * a.rank + j) : 0.0f;
+          acc[r][t] = fmaf(bv, v, acc[r][t]);
+        }
+      }
+    }
+  }
+  pdl_trigger();
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+      if (t < T) {
+        const float s = warp_sum(acc[r][t]);
+        if (lane == (r * TT + t) % 32 && o0 + r < a.N) store_val<XT>(a.y, (size_t)t * a.y_stride + o0 + r, s);
+      }
 }
 
 // ---------------------------------------------------------------- gemm
@@ -270,23 +594,27 @@ constexpr int kLgWarps = 2 + kLgConv + kLgEpi;
 constexpr int kLgThreads = kLgWarps * 32;
 constexpr int kLgMaxN = 256;
 constexpr int kLgGran = kLgMaxN * 8;      // 16-wide pieces of adapters: 256 tokens of rank 128
+constexpr int kLgRO = 4;                  // operand stages (one K group each)
+constexpr int kLgRQ = 4;                  // Q4 tiles (32 rows of one K group) in flight per converter warp
+constexpr int kLgQPitch = 48;             // bytes per row of a Q4 tile: 16-byte reads of 8 rows meet all banks
+constexpr size_t kLgStage = 32768;        // x: 256 tokens of one plane or 128 of two
+constexpr size_t kLgQTile = (size_t)32 * kLgQPitch;
+constexpr uint32_t kLgTmemA = 256;        // below: two sums of 128 tokens or one of 256
 
 template <bool F32>
 struct LgCfg {
-  static constexpr int PL = F32 ? 2 : 1;        // operand planes of W and of x
+  static constexpr int PL = F32 ? 2 : 1;        // planes of x
   static constexpr int NMAX = F32 ? 128 : 256;  // tokens per tile
-  static constexpr int RO = F32 ? 4 : 5;        // operand stages (one K group each)
   static constexpr int GROUP = F32 ? 4 : 1 << 30;  // stages per partial sum
-  static constexpr uint32_t A_COLS = 32 * PL;
-  static constexpr uint32_t TMEM_A = 256;       // below: two sums of 128 tokens or one of 256
-  static constexpr size_t STAGE = (size_t)NMAX * 128 * PL;
+  static constexpr int NV = F32 ? 3 : 2;        // bf16 planes of v
 };
 // Per-tile lists, two buffers: written by the epilogue warps for all roles.
 struct alignas(16) LgList {
   int id[kLgMaxN];          // adapter of each token, -1 none
+  float fx[kLgMaxN];        // 2^exponent of the tokens' rows
   uint16_t first[kLgMaxN];  // first token of the tile with the same adapter, 0xFFFF none
   uint16_t rank[kLgMaxN];
-  int ex[kLgMaxN];          // exponents of the tokens' rows
+  uint16_t goff[kLgMaxN];   // first piece of the adapter, at its first token
   uint16_t gran[kLgGran];   // piece: first token << 4 | index of the 16 rows
   int n_gran;
   int wsum[kLgEpi];
@@ -297,8 +625,9 @@ struct LgShared {
   int bad;                  // some B held a non-finite value
   volatile int abort;
   uint32_t tmem;
-  uint64_t opfull[8], opempty[8], accfull[2], accempty[2], listfull[2], epi;
+  uint64_t opfull[kLgRO], opempty[kLgRO], accfull[2], accempty[2], listfull[2], epi;
 };
+constexpr size_t kLgSmem = kLgRO * kLgStage + kLgConv * kLgRQ * kLgQTile + sizeof(LgShared) + 1024;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -324,55 +653,64 @@ __device__ __forceinline__ int ld_cluster_i(uint32_t addr) {
   return v;
 }
 
-// The exponent of row o of W: of the largest |scale q + bias| its groups allow.
-__device__ __forceinline__ int weight_exponent(const LoraArgs& a, int o) {
-  if (o >= a.N) return 0;
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+// bf16 scales (or biases) of groups 8 k8 .. 8 k8 + 7 of a row, zero behind G
+__device__ __forceinline__ uint4 load_meta(const LoraArgs& a, const uint16_t* base, int o, int k8) {
   const int G = a.K >> 6;
-  const uint16_t* s = a.scales + (size_t)o * G;
-  const uint16_t* b = a.biases + (size_t)o * G;
-  float m = 0.0f;
-  for (int g = 0; g < G; ++g) {
-    const float sc = bf16_bits_to_f32(s[g]), bi = bf16_bits_to_f32(b[g]);
-    m = fmaxf(m, fmaxf(fabsf(bi), fabsf(fmaf(15.0f, sc, bi))));
-  }
-  return row_exponent(m);
+  const uint16_t* s = base + (size_t)o * G + 8 * k8;
+  if (a.m_vec && 8 * k8 + 8 <= G) return __ldg(reinterpret_cast<const uint4*>(s));
+  uint32_t v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 8 * k8 + e < G ? s[e] : 0u;
+  return make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
 }
 
-// What the rows of B of one adapter that are not finite add to y[o] of token t
-// (their places in the matrix product were taken as zero).
-template <int AT>
-__device__ __noinline__ float bad_terms(const LoraArgs& a, int id, int rank, int o, long long t) {
+// Adds to y[t][o] the terms of B's values that are not finite (their places in
+// the matrix product were taken as zero).
+template <int XT, int AT>
+__device__ __noinline__ void add_bad_terms(const LoraArgs& a, int id, int rank, int o, long long t) {
   float s = 0.0f;
+  bool any = false;
   for (int j = 0; j < rank; ++j) {
     const float w = load_val<AT>(a.b, (size_t)id * a.b_stride + (size_t)o * a.rank + j);
-    if (!isfinite(w)) s += w * a.v[(size_t)t * a.v_stride + j];
+    if (!isfinite(w)) {
+      float v = 0.0f;
+      for (int p = a.v_planes - 1; p >= 0; --p)
+        v += bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.v)[((size_t)t * a.v_planes + p) * a.v_stride + j]);
+      s += w * v;
+      any = true;
+    }
   }
-  return s;
+  const size_t at = (size_t)t * a.y_stride + o;
+  if (any) store_val<XT>(a.y, at, load_val<XT>(a.y, at) + s);
 }
 
 template <int XT, int AT>
-__global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs a) {
+__global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_constant__ LoraArgs a) {
   constexpr bool F32 = XT == 0;
   using C = LgCfg<F32>;
   constexpr int PL = C::PL;
   extern __shared__ unsigned char lg_raw[];
   unsigned char* stages = lg_raw + ((1024u - (smem_addr(lg_raw) & 1023u)) & 1023u);
-  LgShared& S = *reinterpret_cast<LgShared*>(stages + C::RO * C::STAGE);
+  unsigned char* qtiles = stages + kLgRO * kLgStage;
+  LgShared& S = *reinterpret_cast<LgShared*>(qtiles + kLgConv * kLgRQ * kLgQTile);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = a.split, rank_c = split > 1 ? (int)cluster_rank() : 0;
   const int mt = (a.N + kLgM - 1) / kLgM, nt = (int)((a.tokens + a.NT - 1) / a.NT);
   const int tiles = mt * nt;
   const int first_tile = split > 1 ? (int)blockIdx.x / split : (int)blockIdx.x;
   const int step = split > 1 ? tiles : (int)gridDim.x;  // a cluster has one tile
-  const int nk = a.K >> 6;
-  const int k_lo = nk * rank_c / split, k_hi = nk * (rank_c + 1) / split, nkm = k_hi - k_lo;
+  // K in stages: nk groups of 64, then the groups' sums against the biases, 64
+  // groups a stage (fp32 rows: the biases' hi and lo parts in two stages)
+  const int nk = a.K >> 6, nbk = (nk + 63) >> 6, nkv = nk + (F32 ? 2 : 1) * nbk;
+  const int k_lo = nkv * rank_c / split, nkm = nkv * (rank_c + 1) / split - k_lo;
+  const int nq = max(0, min(nk - k_lo, nkm));   // of them from Q4 rows
   const int nbuf = a.NT <= 128 ? 2 : 1;
-  // passes over the adapters' pieces: fp32 rows (B hi, lo) x (v0, v1), B x v2;
-  // 16-bit rows B hi x v0, B hi x v1, and for fp16 adapters B lo x v0
-  const int passes = F32 ? 2 : AT == 2 ? 3 : 2;
   volatile int* abort = &S.abort;
   if (tid == 0) {
-    for (int i = 0; i < C::RO; ++i) {
+    for (int i = 0; i < kLgRO; ++i) {
       mbar_init(&S.opfull[i], 5);   // the four warps that wrote the stage, and the producer
       mbar_init(&S.opempty[i], 1);
     }
@@ -395,10 +733,13 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
   fence_after();
   const uint32_t tmem = S.tmem;
   auto tokens_of = [&](int tile) { return (int)min((long long)a.NT, a.tokens - (long long)(tile / mt) * a.NT); };
+  // planes of v that a stage holds, and the passes over the adapters that makes
+  auto v_planes = [&](int npad) { return min(C::NV, 256 / npad); };
+  auto v_passes = [&](int npad) { const int p = v_planes(npad); return (C::NV + p - 1) / p; };
   // stages this CTA adds for the adapters of a tile (its share of the blocks of 64 columns)
-  auto lora_stages = [&](int ng) {
+  auto lora_stages = [&](int ng, int npad) {
     const int nb = (ng + 3) >> 2;
-    return nb > rank_c ? (nb - rank_c + split - 1) / split * passes : 0;
+    return nb > rank_c ? (nb - rank_c + split - 1) / split * v_passes(npad) : 0;
   };
 
   if (warp == 0) {
@@ -410,7 +751,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
       bool ok = true;
       for (int tile = first_tile; tile < tiles && ok; tile += step, ++ti) {
         const int npad = (tokens_of(tile) + 15) & ~15;
-        const unsigned char* src = a.planes + (size_t)(tile / mt) * nk * PL * a.NT * 128;
+        const unsigned char* src = a.planes + (size_t)(tile / mt) * (nk + nbk) * PL * a.NT * 128;
         int total = nkm;
         for (int c = 0; c < total; ++c, ++os) {
           if (c == nkm - 1) {
@@ -418,19 +759,20 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
               ok = false;
               break;
             }
-            total += lora_stages(S.list[ti & 1].n_gran);
+            total += lora_stages(S.list[ti & 1].n_gran, npad);
           }
-          const int st = (int)(os % C::RO);
-          if (os >= (uint32_t)C::RO && !tc_wait(&S.opempty[st], ((os / C::RO) - 1) & 1, abort, a.status)) {
+          const int st = (int)(os % kLgRO);
+          if (os >= (uint32_t)kLgRO && !tc_wait(&S.opempty[st], ((os / kLgRO) - 1) & 1, abort, a.status)) {
             ok = false;
             break;
           }
           if (c < nkm) {
-            unsigned char* dst = stages + (size_t)st * C::STAGE;
+            unsigned char* dst = stages + (size_t)st * kLgStage;
+            const int k = k_lo + c, kp = k < nk ? k : nk + (F32 ? (k - nk) >> 1 : k - nk);
             mbar_arrive_expect(&S.opfull[st], (uint32_t)(PL * npad * 128));
 #pragma unroll
             for (int p = 0; p < PL; ++p)
-              bulk_load(dst + (size_t)p * C::NMAX * 128, src + ((size_t)(k_lo + c) * PL + p) * a.NT * 128,
+              bulk_load(dst + (size_t)p * C::NMAX * 128, src + ((size_t)kp * PL + p) * a.NT * 128,
                         (uint32_t)(npad * 128), &S.opfull[st]);
           } else {
             mbar_arrive(&S.opfull[st]);
@@ -439,8 +781,8 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
       }
       // no copy may still be landing when the CTA ends
       if (!ok)
-        for (uint32_t i = os > (uint32_t)C::RO ? os - C::RO : 0; i < os; ++i)
-          for (int n = 0; n < 1 << 16 && !mbar_test(&S.opfull[i % C::RO], (i / C::RO) & 1); ++n) {
+        for (uint32_t i = os > (uint32_t)kLgRO ? os - kLgRO : 0; i < os; ++i)
+          for (int n = 0; n < 1 << 16 && !mbar_test(&S.opfull[i % kLgRO], (i / kLgRO) & 1); ++n) {
           }
     }
     __syncwarp();
@@ -454,6 +796,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
       for (int tile = first_tile; tile < tiles && ok; tile += step, ++ti) {
         const int npad = (tokens_of(tile) + 15) & ~15;
         const uint32_t idf = idesc16(kLgM, npad, false), idb = idesc16(kLgM, npad, true);
+        const int vpl = v_planes(npad), passes = v_passes(npad);
         int total = nkm;
         uint32_t d = 0;
         for (int c = 0; c < total; ++c, ++os) {
@@ -462,7 +805,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
               ok = false;
               break;
             }
-            total += lora_stages(S.list[ti & 1].n_gran);
+            total += lora_stages(S.list[ti & 1].n_gran, npad);
           }
           const int b = nbuf == 2 ? (int)(gq & 1) : 0;
           bool first = c % C::GROUP == 0;
@@ -474,40 +817,32 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
             }
             d = tmem + (uint32_t)(b * 128);
           }
-          const int st = (int)(os % C::RO);
-          if (!tc_wait(&S.opfull[st], (os / C::RO) & 1, abort, a.status)) {
+          const int st = (int)(os % kLgRO);
+          if (!tc_wait(&S.opfull[st], (os / kLgRO) & 1, abort, a.status)) {
             ok = false;
             break;
           }
           fence_after();
-          const uint32_t ab = tmem + C::TMEM_A + (uint32_t)st * C::A_COLS;
-          const uint64_t bd = bdesc0 + (uint64_t)st * (C::STAGE >> 4);
-          auto issue = [&](int pa, int pb, uint32_t id) {
+          const uint32_t ab = tmem + kLgTmemA + (uint32_t)st * 64;
+          const uint64_t bd = bdesc0 + (uint64_t)st * (kLgStage >> 4);
+          auto issue = [&](int pa, uint32_t boff, uint32_t id) {
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-              mma_ts(d, ab + (uint32_t)(pa * 32 + ks * 8),
-                     bd + (uint64_t)(((size_t)pb * C::NMAX * 128 + ks * 32) >> 4), id, first && ks == 0 ? 0u : 1u);
-            }
+            for (int ks = 0; ks < 4; ++ks)
+              mma_ts(d, ab + (uint32_t)(pa * 32 + ks * 8), bd + (uint64_t)((boff + ks * 32) >> 4), id,
+                     first && ks == 0 ? 0u : 1u);
             first = false;
           };
           if (c < nkm) {
             issue(0, 0, idf);
-            if constexpr (F32) {
-              issue(0, 1, idf);
-              issue(1, 0, idf);
-            }
-          } else if constexpr (F32) {
-            const int pass = (c - nkm) % passes;
-            issue(0, 0, idb);
-            if (pass == 0) {
-              issue(0, 1, idb);
-              if (AT == 2) {
-                issue(1, 0, idb);
-                issue(1, 1, idb);
-              }
-            }
+            // the lo part of x; not for the lo part of the biases
+            if (F32 && (k_lo + c < nk || ((k_lo + c - nk) & 1) == 0)) issue(0, (uint32_t)C::NMAX * 128, idf);
           } else {
-            issue(0, 0, idb);
+            const int p0 = (c - nkm) % passes * vpl;
+            for (int p = 0; p < vpl && p0 + p < C::NV; ++p) {
+              issue(0, (uint32_t)(p * npad * 128), idb);
+              // fp16 adapters: the lo part of B against all but the last plane of v
+              if (AT == 2 && p0 + p < C::NV - 1) issue(1, (uint32_t)(p * npad * 128), idb);
+            }
           }
           commit(&S.opempty[st]);
           if (c % C::GROUP == C::GROUP - 1 || c == total - 1) {
@@ -519,199 +854,268 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
     }
     __syncwarp();
   } else if (warp < 2 + kLgConv) {
-    // ---------------- converters ----------------
-    const int grp = (warp - 2) >> 2;         // stages with os % 2 == grp
+    // ---------------- converters: group 0 the even stages of a tile, group 1 the odd ones ----------------
+    const int grp = (warp - 2) >> 2;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;        // tensor-memory lane = row of the tile
     const int gt = ((warp - 2) & 3) * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-    const int G = nk;
-    struct Raw {
-      uint4 w0, w1;
-      uint32_t s, b;
-    };
-    auto load_raw = [&](int tile, int c, Raw& r) {
-      const int o = (tile % mt) * kLgM + row;
-      if (o >= a.N) {
-        r.w0 = r.w1 = make_uint4(0, 0, 0, 0);
-        r.s = r.b = 0;
-        return;
+    unsigned char* ring = qtiles + (size_t)(warp - 2) * kLgRQ * kLgQTile;
+    // Q4 tiles of this warp's stages, kLgRQ of them ahead: 16 bytes per lane and
+    // copy, two lanes per row
+    int f_tile = grp < nq ? first_tile : tiles, f_c = grp;
+    uint32_t f_n = 0, used = 0;
+    const uint32_t* f_src[2];                // this lane's two pieces, null behind the last row
+    auto f_rows = [&]() {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = (f_tile % mt) * kLgM + quad * 32 + (lane >> 1) + 16 * i;
+        f_src[i] = f_tile < tiles && r < a.N
+                       ? a.packed + (size_t)r * (a.K >> 3) + (size_t)(k_lo + grp) * 8 + (lane & 1) * 4 : nullptr;
       }
-      const int k = k_lo + c;
-      const uint32_t* p = a.packed + (size_t)o * (a.K >> 3) + k * 8;
-      if (a.w_vec) {
-        r.w0 = __ldg(reinterpret_cast<const uint4*>(p));
-        r.w1 = __ldg(reinterpret_cast<const uint4*>(p) + 1);
-      } else {
-        r.w0 = make_uint4(p[0], p[1], p[2], p[3]);
-        r.w1 = make_uint4(p[4], p[5], p[6], p[7]);
-      }
-      r.s = a.scales[(size_t)o * G + k];
-      r.b = a.biases[(size_t)o * G + k];
     };
-    uint32_t os = 0;
+    f_rows();
+    auto fetch = [&]() {
+      if (f_tile < tiles) {
+        unsigned char* to = ring + (f_n % kLgRQ) * kLgQTile + (lane >> 1) * kLgQPitch + (lane & 1) * 16;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (f_src[i] == nullptr) continue;
+          if (a.w_vec)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to + i * 16 * kLgQPitch)),
+                         "l"(f_src[i]) : "memory");
+          else
+            *reinterpret_cast<uint4*>(to + i * 16 * kLgQPitch) =
+                make_uint4(f_src[i][0], f_src[i][1], f_src[i][2], f_src[i][3]);
+          f_src[i] += 16;
+        }
+        f_c += 2;
+        if (f_c >= nq) {
+          f_tile += step;
+          f_c = grp;
+          f_rows();
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      ++f_n;
+    };
+    for (int i = 0; i < kLgRQ; ++i) fetch();
+    pdl_wait();
+    uint32_t os = 0;                         // stages before this tile
     int ti = 0;
-    bool ok = true, waited = false;
+    bool ok = true;
     for (int tile = first_tile; tile < tiles && ok; tile += step, ++ti) {
-      const int o = (tile % mt) * kLgM + row;
-      // this group's stages of the tile: c = c0, c0 + 2, ...
-      const int c0 = (int)((os ^ (uint32_t)grp) & 1u);
-      Raw cur, nxt;
-      if (c0 < nkm) load_raw(tile, c0, cur);
-      if (c0 + 2 < nkm) load_raw(tile, c0 + 2, nxt);
-      const int ew = weight_exponent(a, o);
-      const float wsc = pow2(-ew);
+      const int m_tile = tile % mt, o = m_tile * kLgM + row;
+      const bool live = o < a.N;
+      const float wsc = pow2(-a.ew[o]);
       const LgList& L = S.list[ti & 1];
+      const int npad = (tokens_of(tile) + 15) & ~15, vpl = v_planes(npad), passes = v_passes(npad);
       int total = nkm, ng = 0;
       bool listed = false;
-      const int npad = (tokens_of(tile) + 15) & ~15;
-      for (int c = c0; ok; c += 2) {
+      uint4 meta = make_uint4(0, 0, 0, 0), meta_n = meta;
+      int m8 = -1;
+      auto slot_free = [&](uint32_t oc) {
+        if (oc >= (uint32_t)kLgRO && !warp_wait(&S.opempty[oc % kLgRO], ((oc / kLgRO) - 1) & 1, abort, a.status))
+          return false;
+        fence_after();
+        return true;
+      };
+      for (int c = grp;; c += 2) {
         if (c >= nkm && !listed) {
           if (!warp_wait(&S.listfull[ti & 1], (ti >> 1) & 1, abort, a.status)) {
             ok = false;
             break;
           }
           ng = L.n_gran;
-          total = nkm + lora_stages(ng);
+          total = nkm + lora_stages(ng, npad);
           listed = true;
         }
         if (c >= total) break;
         const uint32_t oc = os + (uint32_t)c;
-        const int st = (int)(oc % C::RO);
-        if (oc >= (uint32_t)C::RO && !warp_wait(&S.opempty[st], ((oc / C::RO) - 1) & 1, abort, a.status)) {
-          ok = false;
-          break;
-        }
-        fence_after();
-        const uint32_t ab = tmem + lane_addr + C::TMEM_A + (uint32_t)st * C::A_COLS;
+        const int st = (int)(oc % kLgRO);
+        const uint32_t ab = tmem + lane_addr + kLgTmemA + (uint32_t)st * 64;
         if (c < nkm) {
-          const uint32_t wv[8] = {cur.w0.x, cur.w0.y, cur.w0.z, cur.w0.w, cur.w1.x, cur.w1.y, cur.w1.z, cur.w1.w};
-          const float s = bf16_bits_to_f32(cur.s) * wsc, bi = bf16_bits_to_f32(cur.b) * wsc;
-          cur = nxt;
-          if (c + 4 < nkm) load_raw(tile, c + 4, nxt);
-          if constexpr (F32) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              uint32_t hi[16], lo[16];
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                  const uint32_t word = wv[half * 4 + w] >> (8 * p);
-                  const float f0 = fmaf(s, (float)(word & 15u), bi), f1 = fmaf(s, (float)((word >> 4) & 15u), bi);
-                  const __half2 h = __floats2half2_rn(f0, f1);
-                  const float2 b2 = __half22float2(h);
-                  hi[4 * w + p] = h2u(h);
-                  lo[4 * w + p] = h2u(__floats2half2_rn(f0 - b2.x, f1 - b2.y));
-                }
-              }
-              st16(ab + (uint32_t)(half * 16), hi);
-              st16(ab + (uint32_t)(32 + half * 16), lo);
+          uint32_t av[32];
+          if (c < nq) {
+            const int k = k_lo + c;
+            if (live && (k >> 3) != m8) {
+              meta = m8 >= 0 && (k >> 3) == m8 + 1 ? meta_n : load_meta(a, a.scales, o, k >> 3);
+              m8 = k >> 3;
+              if ((m8 + 1) * 8 < nk) meta_n = load_meta(a, a.scales, o, m8 + 1);
             }
-          } else {
-            const __half2 s2 = __float2half2_rn(s), b2 = __float2half2_rn(bi), k1024 = u2h(0x64006400u);
-            uint32_t av[32];
+            asm volatile("cp.async.wait_group %0;" ::"n"(kLgRQ - 1) : "memory");
+            __syncwarp();                    // the other lanes' copies too
+            const unsigned char* q = ring + (used % kLgRQ) * kLgQTile + lane * kLgQPitch;
+            const uint4 w0 = *reinterpret_cast<const uint4*>(q), w1 = *reinterpret_cast<const uint4*>(q + 16);
+            ++used;
+            __syncwarp();                    // read by all lanes before the tile is filled again
+            fetch();
+            const uint32_t wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+            const uint32_t sw = word_of(meta, (k >> 1) & 3);
+            // scale (q - 8), at most 8 + 3 significant bits and so exact in fp16:
+            // a nibble in the mantissa of 16.0 is 16 + q, and 24 scale is exact too.
+            // The pairs are (q_i, q_i+4) of a word; x is laid out alike.
+            const __half2 s2 = __float2half2_rn((k & 1 ? bf_hi(sw) : bf_lo(sw)) * wsc),
+                          m24 = __hmul2(s2, __float2half2_rn(-24.0f));
 #pragma unroll
             for (int w = 0; w < 8; ++w) {
-              const uint32_t l = wv[w] & 0x0F0F0F0Fu, h = (wv[w] >> 4) & 0x0F0F0F0Fu;
+              const uint32_t v[4] = {wv[w] << 6, wv[w] << 2, wv[w] >> 2, wv[w] >> 6};
 #pragma unroll
               for (int p = 0; p < 4; ++p)
-                av[4 * w + p] = h2u(__hfma2(__hsub2(u2h(nib_pair(l, h, p) | 0x64006400u), k1024), s2, b2));
+                av[4 * w + p] = h2u(__hfma2(u2h((v[p] & 0x03C003C0u) | 0x4C004C00u), s2, m24));
             }
-            st32(ab, av);
+          } else {
+            // the biases of 64 groups
+            const uint32_t* b = a.wbias + ((size_t)m_tile * (nkv - nk) + (size_t)(k_lo + c - nk)) * 32 * 128 + row;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) av[e] = __ldg(b + e * 128);
           }
+          if (!slot_free(oc)) {
+            ok = false;
+            break;
+          }
+          st32(ab, av);
         } else {
           // a block of 64 columns: four pieces of 16 rows of adapters
-          if (!waited) {
-            pdl_wait();
-            waited = true;
-          }
-          const int lc = c - nkm, blk = rank_c + lc / passes * split, pass = lc % passes;
+          const int lc = c - nkm, blk = rank_c + lc / passes * split, p0 = lc % passes * vpl;
+          int left[4];                       // rows of the adapter from this piece on, 0: no piece
+          uint4 raw[4][2];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const int gi = blk * 4 + q;
-            const int gr = gi < ng ? L.gran[gi] : 0xFFFF;
-            uint32_t hi[8] = {}, lo[8] = {};
-            if (gr != 0xFFFF && o < a.N) {
-              const int id = L.id[gr >> 4], rank = L.rank[gr >> 4], j0 = (gr & 15) * 16;
-              const size_t at = (size_t)id * a.b_stride + (size_t)o * a.rank + j0;
-              float w[16];
+            const int gr = blk * 4 + q < ng ? (int)L.gran[blk * 4 + q] : 0xFFFF;
+            raw[q][0] = raw[q][1] = make_uint4(0, 0, 0, 0);
+            left[q] = 0;
+            if (gr != 0xFFFF && live) {
+              const int j0 = (gr & 15) * 16;
+              left[q] = (int)L.rank[gr >> 4] - j0;
+              const uint16_t* at = static_cast<const uint16_t*>(a.b) + (size_t)L.id[gr >> 4] * a.b_stride +
+                                   (size_t)o * a.rank + j0;
               if (a.b_vec && j0 + 16 <= a.rank) {
-                float w0[8], w1[8];
-                load8<AT>(a.b, at, true, w0);
-                load8<AT>(a.b, at + 8, true, w1);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  w[e] = j0 + e < rank ? w0[e] : 0.0f;
-                  w[8 + e] = j0 + 8 + e < rank ? w1[e] : 0.0f;
-                }
+                raw[q][0] = __ldg(reinterpret_cast<const uint4*>(at));
+                raw[q][1] = __ldg(reinterpret_cast<const uint4*>(at) + 1);
               } else {
+                uint32_t h[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) w[e] = j0 + e < rank ? load_val<AT>(a.b, at + e) : 0.0f;
+                for (int e = 0; e < 16; ++e) h[e] = e < left[q] ? at[e] : 0u;
+                raw[q][0] = make_uint4(pack2(h[0], h[1]), pack2(h[2], h[3]), pack2(h[4], h[5]), pack2(h[6], h[7]));
+                raw[q][1] =
+                    make_uint4(pack2(h[8], h[9]), pack2(h[10], h[11]), pack2(h[12], h[13]), pack2(h[14], h[15]));
               }
-              bool bad = false;
+            }
+          }
+          // this thread's first token: its pieces in the block, the first one's v
+          auto pieces_of = [&](int n, int& q0, int& q1) {
+            const int mine = n < npad ? (int)L.first[n] : 0xFFFF;
+            q0 = q1 = 4;
+            if (mine != 0xFFFF) {
+              const int g0 = (int)L.goff[mine] - blk * 4, g1 = g0 + (((int)L.rank[n] + 15) >> 4);
+              q0 = max(0, min(4, g0));
+              q1 = max(0, min(4, g1));
+            }
+            return (blk * 4 - (mine != 0xFFFF ? (int)L.goff[mine] : 0)) * 16;   // column 0 of the block, in its v
+          };
+          const long long tn = (long long)(tile / mt) * a.NT;
+          int q0, q1;
+          int j0 = pieces_of(gt, q0, q1);
+          // the planes of this pass, 16 columns each
+          uint4 f[C::NV][2];
+          const uint16_t* vp = reinterpret_cast<const uint16_t*>(a.v) + (size_t)p0 * a.v_stride;
+          auto load_v = [&](int n, int j) {
+            const uint16_t* at = vp + (size_t)(tn + n) * C::NV * a.v_stride + j;
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                if (!isfinite(w[e])) {
-                  bad = true;
-                  w[e] = 0.0f;
-                }
-                w[e] *= wsc;
+            for (int p = 0; p < C::NV; ++p)
+              if (p < vpl && p0 + p < C::NV) {
+                f[p][0] = *reinterpret_cast<const uint4*>(at + (size_t)p * a.v_stride);
+                f[p][1] = *reinterpret_cast<const uint4*>(at + (size_t)p * a.v_stride + 8);
               }
-              if (bad) S.bad = 1;
+          };
+          int ex = 0;
+          if (q0 < q1) {
+            ex = a.ex[tn + gt];
+            load_v(gt, j0 + q0 * 16);
+          }
+          if (!slot_free(oc)) {
+            ok = false;
+            break;
+          }
+          // ---- B ----
+          const uint32_t wsc2 = pack_bf2(wsc, wsc);
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t w[8] = {raw[q][0].x, raw[q][0].y, raw[q][0].z, raw[q][0].w,
+                             raw[q][1].x, raw[q][1].y, raw[q][1].z, raw[q][1].w};
+            if (left[q] < 16) {
+#pragma unroll
+              for (int p = 0; p < 8; ++p)
+                w[p] &= (2 * p < left[q] ? 0xFFFFu : 0u) | (2 * p + 1 < left[q] ? 0xFFFF0000u : 0u);
+            }
+            // a non-finite value must not meet the zeros of other tokens: an
+            // exponent of all ones carries into the sign place
+            constexpr uint32_t kExp = AT == 2 ? 0x7C007C00u : 0x7F807F80u, kOne = AT == 2 ? 0x04000400u : 0x00800080u;
+            uint32_t any = 0;
+#pragma unroll
+            for (int p = 0; p < 8; ++p) any |= (w[p] & kExp) + kOne;
+            if (any & 0x80008000u) {
+              S.bad = 1;
 #pragma unroll
               for (int p = 0; p < 8; ++p) {
-                hi[p] = pack_bf2(w[2 * p], w[2 * p + 1]);
-                lo[p] = pack_bf2(w[2 * p] - bf_lo(hi[p]), w[2 * p + 1] - bf_hi(hi[p]));
+                const uint32_t b = ((w[p] & kExp) + kOne) & 0x80008000u;
+                w[p] &= ~((b >> 15) * 0xFFFFu);
               }
             }
             __syncwarp();
-            if constexpr (F32) {
+            if constexpr (AT == 2) {
+              uint32_t hi[8], lo[8];
+#pragma unroll
+              for (int p = 0; p < 8; ++p) {
+                float w0, w1;
+                unpack2<AT>(w[p], w0, w1);
+                w0 *= wsc;
+                w1 *= wsc;
+                hi[p] = pack_bf2(w0, w1);
+                lo[p] = pack_bf2(w0 - bf_lo(hi[p]), w1 - bf_hi(hi[p]));
+              }
               st8(ab + (uint32_t)(q * 8), hi);
               st8(ab + (uint32_t)(32 + q * 8), lo);
             } else {
-              if (pass == 2) st8(ab + (uint32_t)(q * 8), lo);
-              else st8(ab + (uint32_t)(q * 8), hi);
+#pragma unroll
+              for (int p = 0; p < 8; ++p) w[p] = bf2_fma(w[p], wsc2, 0x80008000u);   // a power of two: exact
+              st8(ab + (uint32_t)(q * 8), w);
             }
           }
-          unsigned char* dst = stages + (size_t)st * C::STAGE;
+          unsigned char* dst = stages + (size_t)st * kLgStage;
+          // ---- v: zeros, and in each token's columns its own planes ----
           for (int n = gt; n < npad; n += 128) {
-            const int mine = L.first[n];
-            const long long t = (long long)(tile / mt) * a.NT + n;
-            const float xsc = mine != 0xFFFF ? pow2(-a.ex[t]) : 0.0f;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int gi = blk * 4 + q;
-              const int gr = gi < ng ? L.gran[gi] : 0xFFFF;
-              uint32_t p0[8] = {}, p1[8] = {};
-              if (gr != 0xFFFF && (gr >> 4) == mine) {
-                const float4* v = reinterpret_cast<const float4*>(a.v + (size_t)t * a.v_stride + (gr & 15) * 16);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float4 f4 = v[e];
-                  const float f[4] = {f4.x * xsc, f4.y * xsc, f4.z * xsc, f4.w * xsc};
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const uint32_t v0 = pack_bf2(f[2 * h], f[2 * h + 1]);
-                    const float r0 = f[2 * h] - bf_lo(v0), r1 = f[2 * h + 1] - bf_hi(v0);
-                    const uint32_t v1 = pack_bf2(r0, r1);
-                    if constexpr (F32) {
-                      const uint32_t v2 = pack_bf2(r0 - bf_lo(v1), r1 - bf_hi(v1));
-                      p0[2 * e + h] = pass == 0 ? v0 : v2;
-                      p1[2 * e + h] = v1;
-                    } else {
-                      p0[2 * e + h] = pass == 1 ? v1 : v0;
-                    }
-                  }
-                }
+            if (n != gt) {
+              j0 = pieces_of(n, q0, q1);
+              if (q0 < q1) {
+                ex = a.ex[tn + n];
+                load_v(n, j0 + q0 * 16);
               }
+            }
+            unsigned char* at = dst + (size_t)n * 128;
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+            const float xsc = pow2(-ex);
+            const uint32_t xsc2 = pack_bf2(xsc, xsc);   // a power of two: exact
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                unsigned char* at = dst + (size_t)n * 128 + (((2 * q + u) ^ (n & 7)) << 4);
-                *reinterpret_cast<uint4*>(at) = make_uint4(p0[4 * u], p0[4 * u + 1], p0[4 * u + 2], p0[4 * u + 3]);
-                if constexpr (F32)
-                  *reinterpret_cast<uint4*>(at + (size_t)C::NMAX * 128) =
-                      make_uint4(p1[4 * u], p1[4 * u + 1], p1[4 * u + 2], p1[4 * u + 3]);
+            for (int p = 0; p < C::NV; ++p) {
+              if (p >= vpl || p0 + p >= C::NV) continue;
+#pragma unroll
+              for (int u = 0; u < 8; ++u)
+                if ((u >> 1) < q0 || (u >> 1) >= q1)
+                  *reinterpret_cast<uint4*>(at + (size_t)p * npad * 128 + ((u ^ (n & 7)) << 4)) = zero;
+            }
+            for (int q = q0; q < q1; ++q) {
+              if (q != q0) load_v(n, j0 + q * 16);
+#pragma unroll
+              for (int p = 0; p < C::NV; ++p) {
+                if (p >= vpl || p0 + p >= C::NV) continue;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                  *reinterpret_cast<uint4*>(at + (size_t)p * npad * 128 + (((2 * q + u) ^ (n & 7)) << 4)) =
+                      make_uint4(bf2_fma(f[p][u].x, xsc2, 0x80008000u), bf2_fma(f[p][u].y, xsc2, 0x80008000u),
+                                 bf2_fma(f[p][u].z, xsc2, 0x80008000u), bf2_fma(f[p][u].w, xsc2, 0x80008000u));
               }
             }
           }
@@ -723,12 +1127,9 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
         if (lane == 0) mbar_arrive(&S.opfull[st]);
       }
       if (!ok) break;
-      if (!listed) {
-        if (!warp_wait(&S.listfull[ti & 1], (ti >> 1) & 1, abort, a.status)) break;
-        total = nkm + lora_stages(L.n_gran);
-      }
       os += (uint32_t)total;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     // ---------------- epilogue ----------------
     const int quad = warp & 3, half = (warp - 2 - kLgConv) >> 2;
@@ -783,27 +1184,49 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
         if (w < warp - 2 - kLgConv) base += L.wsum[w];
         all += L.wsum[w];
       }
+      L.goff[n_mine] = (uint16_t)(base + incl - mine);
       for (int i = 0; i < mine; ++i) L.gran[base + incl - mine + i] = (uint16_t)(n_mine << 4 | i);
       if (n_mine == 0) L.n_gran = all;
       __syncwarp();
       if (lane == 0) mbar_arrive(&S.listfull[ti & 1]);
       if (ti == 0) pdl_wait();  // what the prep kernel wrote; y may still be read before it
-      L.ex[n_mine] = n_mine < ntok ? a.ex[tb + n_mine] : 0;
-      const int ew = weight_exponent(a, o);
+      const int ew = a.ew[o];
       if (half == 0) S.ew[row] = ew;
+      L.fx[n_mine] = n_mine < ntok ? pow2(a.ex[tb + n_mine]) : 0.0f;
       if (!meet()) break;
-      const int total = nkm + lora_stages(all);
+      const int total = nkm + lora_stages(all, npad);
       const bool live = o < a.N;
       float* part = reinterpret_cast<float*>(stages);  // split: [token][128 rows]
-      auto put = [&](int n, float v) {
-        v = scale_by(v, ew + L.ex[n]);
-        if (S.bad && L.first[n] != 0xFFFF) v += bad_terms<AT>(a, L.id[n], L.rank[n], o, tb + n);
-        store_val<XT>(a.y, (size_t)(tb + n) * a.y_stride + o, v);
+      // a sum times 2^(ew + ex): within range in this order, as |ew| above 60
+      // is taken in two steps
+      const int ewc = max(-60, min(60, ew));
+      const float fw = pow2(ewc), fr = pow2(ew - ewc);
+      // 16 columns of sums to y
+      auto put16 = [&](int n0, const float (&v)[16]) {
+        if (!live) return;
+        float fx[16];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4 f = *reinterpret_cast<const float4*>(&L.fx[n0 + 4 * e]);
+          fx[4 * e] = f.x;
+          fx[4 * e + 1] = f.y;
+          fx[4 * e + 2] = f.z;
+          fx[4 * e + 3] = f.w;
+        }
+        const size_t at = (size_t)(tb + n0) * a.y_stride + o;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float r = v[e] * fw * fx[e];
+          if (ew != ewc) r *= fr;
+          if (n0 + e < ntok) store_val<XT>(a.y, at + (size_t)e * a.y_stride, r);
+        }
       };
       if constexpr (F32) {
-        float acc[64];
+        float acc[4][16];
 #pragma unroll
-        for (int e = 0; e < 64; ++e) acc[e] = 0.0f;
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
         bool ok = true;
         for (int c = 0; c < total; c += C::GROUP, ++gq) {
           const int b = (int)(gq & 1);
@@ -814,13 +1237,13 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
           fence_after();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int c0 = (2 * i + half) * 16;
-            if (c0 < npad) {
+            const int n0 = (2 * i + half) * 16;
+            if (n0 < npad) {
               uint32_t d[16];
-              ld16(tmem + lane_addr + (uint32_t)(b * 128 + c0), d);
+              ld16(tmem + lane_addr + (uint32_t)(b * 128 + n0), d);
               wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) acc[i * 16 + e] += __uint_as_float(d[e]);
+              for (int e = 0; e < 16; ++e) acc[i][e] += __uint_as_float(d[e]);
             }
           }
           fence_before();
@@ -830,14 +1253,13 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
         if (!ok) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+          const int n0 = (2 * i + half) * 16;
+          if (n0 >= npad) continue;
+          if (split > 1) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int n = (2 * i + half) * 16 + e;
-            if (split > 1) {
-              if (n < npad) part[n * kLgM + row] = acc[i * 16 + e];
-            } else if (live && n < ntok) {
-              put(n, acc[i * 16 + e]);
-            }
+            for (int e = 0; e < 16; ++e) part[(n0 + e) * kLgM + row] = acc[i][e];
+          } else {
+            put16(n0, acc[i]);
           }
         }
       } else {
@@ -845,21 +1267,28 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
         if (!warp_wait(&S.accfull[b], (nbuf == 2 ? gq >> 1 : gq) & 1, abort, a.status)) break;
         fence_after();
         ++gq;
-        for (int c0 = half * 16; c0 < npad; c0 += 32) {
+        for (int n0 = half * 16; n0 < npad; n0 += 32) {
           uint32_t d[16];
-          ld16(tmem + lane_addr + (uint32_t)(b * 128 + c0), d);
+          ld16(tmem + lane_addr + (uint32_t)(b * 128 + n0), d);
           wait_ld();
+          float v[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int n = c0 + e;
-            if (split > 1) part[n * kLgM + row] = __uint_as_float(d[e]);
-            else if (live && n < ntok) put(n, __uint_as_float(d[e]));
+          for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(d[e]);
+          if (split > 1) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) part[(n0 + e) * kLgM + row] = v[e];
+          } else {
+            put16(n0, v);
           }
         }
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.accempty[b]);
       }
+      // terms that are not finite, after the fact: they decide their values
+      if (S.bad && split == 1 && live)
+        for (int n = half * 16; n < ntok; n += (n & 15) == 15 ? 17 : 1)
+          if (L.first[n] != 0xFFFF) add_bad_terms<XT, AT>(a, L.id[n], L.rank[n], o, tb + n);
     }
   }
   if (split > 1) {
@@ -876,11 +1305,16 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
       const int n = n_lo + i / kLgM, row = i % kLgM, o = (tile % mt) * kLgM + row;
       if (o >= a.N || S.abort) continue;
       const uint32_t at = smem_addr(stages) + (uint32_t)(n * kLgM + row) * 4;
-      float v = 0.0f;
-      for (int r = 0; r < split; ++r) v += ld_cluster(map_rank(at, (uint32_t)r));
-      v = scale_by(v, S.ew[row] + L.ex[n]);
-      if (bad && L.first[n] != 0xFFFF) v += bad_terms<AT>(a, L.id[n], L.rank[n], o, tb + n);
+      float p[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) p[r] = r < split ? ld_cluster(map_rank(at, (uint32_t)r)) : 0.0f;
+      float v = p[0];
+#pragma unroll
+      for (int r = 1; r < 8; ++r) v += p[r];
+      const int ew = S.ew[row], ewc = max(-60, min(60, ew));
+      v = v * pow2(ewc) * L.fx[n] * pow2(ew - ewc);
       store_val<XT>(a.y, (size_t)(tb + n) * a.y_stride + o, v);
+      if (bad && L.first[n] != 0xFFFF) add_bad_terms<XT, AT>(a, L.id[n], L.rank[n], o, tb + n);
     }
     cluster_sync_all();  // no CTA ends while another reads its sums
   }
@@ -889,15 +1323,18 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const LoraArgs
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
-template <bool F32>
-constexpr size_t lg_smem() {
-  return (size_t)LgCfg<F32>::RO * LgCfg<F32>::STAGE + sizeof(LgShared) + 1024;
+// ---------------------------------------------------------------- launches
+
+bool decodes(const LoraArgs& a) {
+  return a.tokens <= kDecTokens && (size_t)a.tokens * a.K * 4 <= kDecSmem;
 }
 
-// Tokens per tile and CTAs per tile (K split over a cluster): the smallest of
-// a plain estimate in clocks.  A stage costs its matrix steps (N / 2 clocks
-// each) or the conversion of its 128 x 64 weights, whichever is longer; a tile
-// adds its epilogue, a split the exchange of the sums.
+// Tokens per tile and CTAs per tile (K and the adapters split over a cluster):
+// the smallest of a plain estimate in clocks.  A stage costs its matrix steps
+// (N / 2 clocks each, 4 per plane of x) or the conversion of its 128 x 64
+// weights, whichever is longer; a stage of adapters, of which a tile of few
+// tokens may have one for every few tokens, about twice that; a tile adds its
+// epilogue, a split the exchange of the sums.
 void lg_shape(const LoraArgs& a, int sms, int* NT, int* split) {
   const bool f32 = a.x_type == 0;
   const int nmax = f32 ? 128 : 256, nk = a.K >> 6;
@@ -908,11 +1345,18 @@ void lg_shape(const LoraArgs& a, int sms, int* NT, int* split) {
   for (int n = 16; n <= nmax; n += 16) {
     if (n > 16 && n - 16 >= a.tokens) break;
     const long long tiles = mt * ((a.tokens + n - 1) / n);
+    double lora = 0.0;
+    if (a.adapter) {
+      const int nv = f32 ? 3 : 2, per = 256 / n < nv ? 256 / n : nv, passes = (nv + per - 1) / per;
+      const double many = a.tokens <= 512 ? (a.count < n ? a.count : n) : 2.0;
+      lora = passes * (many * ((a.rank + 15) / 16) / 4.0 + 0.5);
+    }
     for (int s = 1; s <= 8; s *= 2) {
       if (s > nk || (s > 1 && tiles * s > (s == 8 ? 128 : sms))) break;
       const double waves = (double)((tiles * s + sms - 1) / sms);
-      const double stage = f32 ? (6.0 * n > 450.0 ? 6.0 * n : 450.0) : (2.0 * n > 220.0 ? 2.0 * n : 220.0);
-      const double t = waves * (((nk + s - 1) / s) * stage + 1500.0 + 12.0 * n + (s > 1 ? 1500.0 : 0.0));
+      const double mma = (f32 ? 4.0 : 2.0) * n, stage = mma > 450.0 ? mma : 450.0;
+      const double t = waves * (((nk + s - 1) / s) * stage + (lora / s) * (2.0 * stage + 300.0) + 1500.0 + 10.0 * n +
+                                (s > 1 ? 1500.0 : 0.0));
       if (t < best) {
         best = t;
         *NT = n;
@@ -923,10 +1367,11 @@ void lg_shape(const LoraArgs& a, int sms, int* NT, int* split) {
 }
 
 template <typename K>
-cudaError_t launch_cfg(K kernel, dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t s, const LoraArgs& a) {
+cudaError_t launch_cfg(K kernel, unsigned grid, unsigned block, size_t smem, int cluster, cudaStream_t s,
+                       const LoraArgs& a) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -944,75 +1389,126 @@ cudaError_t launch_cfg(K kernel, dim3 grid, dim3 block, size_t smem, int cluster
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
+// Rows of W per warp of the decode kernel: more of them share the reads of x
+// from shared memory, fewer leave more warps.
+template <int XT, int AT, int TT>
+cudaError_t launch_decode(const LoraArgs& a, cudaStream_t s) {
+  const size_t sm = (size_t)a.tokens * a.K * 4;
+  if (TT >= 4 && a.N >= 1024)
+    return launch_cfg(lora_decode_kernel<XT, AT, TT, 2>, (unsigned)((a.N + 2 * kDecWarps - 1) / (2 * kDecWarps)),
+                      kDecWarps * 32, sm, 1, s, a);
+  return launch_cfg(lora_decode_kernel<XT, AT, TT, 1>, (unsigned)((a.N + kDecWarps - 1) / kDecWarps), kDecWarps * 32,
+                    sm, 1, s, a);
+}
+
 template <int XT, int AT>
 cudaError_t launch(const LoraArgs& a, int sms, cudaStream_t s, uint64_t* launches) {
-  const unsigned tiles16 = (unsigned)((a.tokens + kPrepRows - 1) / kPrepRows);
-  // blocks per tile for the adapters: up to the 16 a tile can hold, fewer
-  // where the tiles alone fill the GPU
-  unsigned ay = 0;
-  if (a.adapter) {
-    ay = (unsigned)(8 * sms) / tiles16;
-    ay = ay < 1 ? 1 : ay > kPrepRows ? kPrepRows : ay;
-    if (ay > (unsigned)a.count) ay = (unsigned)a.count;
-    if (ay > (unsigned)a.tokens) ay = (unsigned)a.tokens;
+  const bool dec = decodes(a);
+  const long long rows = (a.tokens + 15) / 16 * 16;
+  const long long row_blocks = dec ? 0 : a.row_threads == 32 ? rows / kPrepWarps : rows;
+  const long long prep = a.v_blocks + a.w_blocks + row_blocks;
+  if (prep) {
+    const cudaError_t e = launch_cfg(lora_prep_kernel<XT, AT>, (unsigned)prep, kPrepThreads, 0, 1, s, a);
+    if (e != cudaSuccess) return e;
+    if (launches) *launches += 1;
   }
-  cudaError_t e = launch_cfg(lora_prep_kernel<XT, AT>, dim3(tiles16, 1 + ay), dim3(kPrepWarps * 32), 0, 1, s, a);
-  if (e != cudaSuccess) return e;
+  if (launches) *launches += 1;
+  if (dec) {
+    if (a.tokens == 1) return launch_decode<XT, AT, 1>(a, s);
+    if (a.tokens == 2) return launch_decode<XT, AT, 2>(a, s);
+    if (a.tokens <= 4) return launch_decode<XT, AT, 4>(a, s);
+    return launch_decode<XT, AT, 8>(a, s);
+  }
   const long long tiles = (long long)((a.N + kLgM - 1) / kLgM) * ((a.tokens + a.NT - 1) / a.NT);
   const unsigned grid = (unsigned)(a.split > 1 ? tiles * a.split : tiles < sms ? tiles : sms);
-  e = launch_cfg(lora_gemm_kernel<XT, AT>, dim3(grid), dim3(kLgThreads), lg_smem<XT == 0>(), a.split, s, a);
-  if (launches) *launches += 2;
-  return e;
+  return launch_cfg(lora_gemm_kernel<XT, AT>, grid, kLgThreads, kLgSmem, a.split, s, a);
 }
 
 constexpr size_t kWsAlign = 1024;
 size_t up(size_t v) { return (v + kWsAlign - 1) / kWsAlign * kWsAlign; }
 
-// Tokens per pair of launches: operand planes of at most 256 MB, which keeps
+// Tokens per round of launches: operand planes of at most 256 MB, which keeps
 // the workspace bounded (a multiple of 256 tokens).
 long long block_tokens(const LoraArgs& a) {
   const long long row = (long long)a.K * (a.x_type == 0 ? 4 : 2);
-  long long n = (256ll << 20) / row / 256 * 256;
+  const long long n = (256ll << 20) / row / 256 * 256;
   return n < 256 ? 256 : n;
 }
 
-size_t carve(LoraArgs& a, unsigned char* base) {
-  const long long tiles = (a.tokens + a.NT - 1) / a.NT;
-  const size_t planes = up((size_t)tiles * a.NT * a.K * (a.x_type == 0 ? 4 : 2));
-  const size_t ex = up((size_t)((a.tokens + 15) / 16 * 16) * 4);
-  a.v_stride = a.adapter ? ((size_t)a.rank + 15) / 16 * 16 : 0;
-  a.planes = base;
-  a.ex = reinterpret_cast<int*>(base + planes);
-  a.v = reinterpret_cast<float*>(base + planes + ex);
-  return planes + ex + up((size_t)a.tokens * a.v_stride * 4);
+// The shape of the launches for a.tokens tokens and the workspace they take.
+size_t shape(LoraArgs& a, int sms, unsigned char* base) {
+  const bool dec = decodes(a);
+  size_t off = 0;
+  a.w_blocks = 0;
+  if (!dec) {
+    lg_shape(a, sms, &a.NT, &a.split);
+    const long long tiles = (a.tokens + a.NT - 1) / a.NT, nk = a.K >> 6;
+    a.planes = base;
+    off += up((size_t)tiles * a.NT * (nk + (nk + 63) / 64) * 128 * (a.x_type == 0 ? 2 : 1));
+    a.ex = reinterpret_cast<int*>(base + off);
+    off += up((size_t)((a.tokens + 15) / 16 * 16) * 4);
+    a.row_threads = a.tokens >= 1024 ? 32 : kPrepThreads;
+    a.w_blocks = (a.N + kLgM - 1) / kLgM;
+    a.ew = reinterpret_cast<int*>(base + off);
+    off += up((size_t)a.w_blocks * kLgM * 4);
+    a.wbias = reinterpret_cast<uint32_t*>(base + off);
+    off += up((size_t)a.w_blocks * (a.x_type == 0 ? 2 : 1) * ((nk + 63) / 64) * 32 * kLgM * 4);
+  }
+  a.v_blocks = 0;
+  a.v_stride = 0;
+  a.v_slots = 1;
+  if (a.adapter) {
+    a.v_stride = ((size_t)a.rank + 15) / 16 * 16;
+    // tiles of 16 tokens while a tile's adapters are worth blocks of their own,
+    // of 32 where a prompt's tokens share them
+    a.v_tile = a.tokens >= 1024 ? 32 : 16;
+    a.v_planes = dec ? 0 : a.x_type == 0 ? 3 : 2;
+    const long long vt = (a.tokens + a.v_tile - 1) / a.v_tile;
+    const long long most = a.tokens < a.count ? a.tokens : a.count;
+    if (a.v_tile == 16) a.v_slots = (int)(most < 16 ? most : 16);
+    a.v_blocks = (int)(vt * a.v_slots);
+    a.v = reinterpret_cast<float*>(base + off);
+    off += up((size_t)a.tokens * a.v_stride * (dec ? 4 : 2 * a.v_planes));
+  }
+  return off;
+}
+
+template <int XT, int AT>
+cudaError_t set_smem() {
+  cudaError_t e = cudaFuncSetAttribute(lora_gemm_kernel<XT, AT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLgSmem);
+  auto dec = [&](auto kernel) {
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kDecSmem);
+  };
+  dec(lora_decode_kernel<XT, AT, 1, 1>);
+  dec(lora_decode_kernel<XT, AT, 2, 1>);
+  dec(lora_decode_kernel<XT, AT, 4, 1>);
+  dec(lora_decode_kernel<XT, AT, 8, 1>);
+  dec(lora_decode_kernel<XT, AT, 4, 2>);
+  dec(lora_decode_kernel<XT, AT, 8, 2>);
+  return e;
 }
 
 }  // namespace
 
 cudaError_t init_lora_attributes(int max_smem) {
-  if ((int)lg_smem<true>() > max_smem || (int)lg_smem<false>() > max_smem) return cudaErrorInvalidConfiguration;
-  cudaError_t e = cudaSuccess;
-  auto set = [&](auto kernel, size_t sm) {
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
-  };
-  set(lora_gemm_kernel<0, 1>, lg_smem<true>());
-  set(lora_gemm_kernel<0, 2>, lg_smem<true>());
-  set(lora_gemm_kernel<1, 1>, lg_smem<false>());
-  set(lora_gemm_kernel<1, 2>, lg_smem<false>());
-  set(lora_gemm_kernel<2, 1>, lg_smem<false>());
-  set(lora_gemm_kernel<2, 2>, lg_smem<false>());
+  if ((int)kLgSmem > max_smem) return cudaErrorInvalidConfiguration;
+  cudaError_t e = set_smem<0, 1>();
+  if (e == cudaSuccess) e = set_smem<0, 2>();
+  if (e == cudaSuccess) e = set_smem<1, 1>();
+  if (e == cudaSuccess) e = set_smem<1, 2>();
+  if (e == cudaSuccess) e = set_smem<2, 1>();
+  if (e == cudaSuccess) e = set_smem<2, 2>();
   return e;
 }
 
 size_t lora_workspace(const LoraArgs& args, int sms) {
-  LoraArgs a = args;
-  const long long all = a.tokens, most = block_tokens(a);
+  const long long most = block_tokens(args);
   size_t need = 0;
-  for (long long n : {all < most ? all : most, all % most}) {
+  for (long long n : {args.tokens < most ? args.tokens : most, args.tokens % most}) {
     if (n == 0) continue;
+    LoraArgs a = args;
     a.tokens = n;
-    lg_shape(a, sms, &a.NT, &a.split);
-    const size_t b = carve(a, nullptr);
+    const size_t b = shape(a, sms, nullptr);
     need = b > need ? b : need;
   }
   return need;
@@ -1030,10 +1526,10 @@ cudaError_t launch_lora(const LoraArgs& args, void* workspace, int sms, cudaStre
     a.x = static_cast<const unsigned char*>(args.x) + (size_t)t0 * args.x_stride * ts;
     a.y = static_cast<unsigned char*>(args.y) + (size_t)t0 * args.y_stride * ts;
     if (a.adapter) a.adapter = args.adapter + t0;
-    lg_shape(a, sms, &a.NT, &a.split);
-    carve(a, static_cast<unsigned char*>(workspace));
-    a.x_vec = aligned(a.x, a.x_stride * ts);
+    shape(a, sms, static_cast<unsigned char*>(workspace));
+    a.x_vec = aligned(a.x, a.tokens > 1 ? a.x_stride * ts : 0);
     a.w_vec = aligned(a.packed, 0);
+    a.m_vec = aligned(a.scales, (size_t)(a.K / 64) * 2) && aligned(a.biases, 0);
     a.a_vec = a.adapter && aligned(a.a, a.a_stride * 2);
     a.b_vec = a.adapter && aligned(a.b, a.b_stride * 2 | (size_t)a.rank * 2);
     cudaError_t e;

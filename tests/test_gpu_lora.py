@@ -1,13 +1,16 @@
 """Context.q4_gemv_lora (osm_q4_gemv_lora) against the definition in 64 bits.
 
-Tolerance, per value y[t][o], with S = sum |w| |x| and L = |gain| sum_j |B_oj|
-sum_k |A_jk| |x_k|:
+Tolerance, per value y[t][o].  With c = bias + 8 scale of each group,
+  S = sum_g sum_k (|scale| |q - 8| + |c|) |x_k|,  C = sum_g |c| sum_k |x_k|,
+  L = |gain| sum_j |B_oj| sum_k |A_jk| |x_k|
+the sum is taken as scale (q - 8) x + c (sum of x per group):
   half a step of y's type times |y| (one rounding at the end);
-  fp32 rows: operands to 2^-22 of themselves, sums in steps of 16 products
-  that each lose at most 2^-23 of the running sum of magnitudes:
-  (3 K / 16 + 8) 2^-23 (S + L), plus rank 2^-23 L;
-  16-bit rows: the weights to half a step of fp16, 2^-12 of the row's largest
-  |w| or of w, the low-rank products to 2^-16: 2^-12 S + 2^-15 L on top.
+  every kind of row: operands to 2^-22 of themselves, a group's sum of x to
+  10 half-ulps, steps of 16 products that each lose at most 2^-23 of the sum of
+  magnitudes, twice over K / 16 steps and three times over K / 1024:
+  (K / 8 + K / 256 + 16) 2^-23 (S + L), plus rank 2^-23 L;
+  16-bit rows: c and the group sums once to fp16, the low-rank products to 16
+  bits: 2^-11 C + 2^-15 L on top.
 """
 import ctypes
 
@@ -75,22 +78,27 @@ class Case:
                 + self.biases.double().repeat_interleave(64, 1))
 
     def reference(self, torch, lora=True):
-        """(y, S, L) in 64 bits."""
+        """(y, (S, C), L) in 64 bits."""
         w, x = self.weight(torch), self.x.double()
-        y, S, L = x @ w.T, x.abs() @ w.abs().T, torch.zeros(self.T, self.N, dtype=torch.float64, device="cuda")
+        L = torch.zeros(self.T, self.N, dtype=torch.float64, device="cuda")
+        c = (self.biases.double() + 8 * self.scales.double()).repeat_interleave(64, 1)
+        y, C = x @ w.T, x.abs() @ c.abs().T
+        S = x.abs() @ (w - c).abs().T + C
         for i in range(self.n if lora else 0):
             rows = (self.adapter == i).nonzero()[:, 0]
             r = self.rank if self.ranks is None else int(self.ranks[i].clamp(max=self.rank))
             a, b, g = self.a[i, :r].double(), self.b[i, :, :r].double(), float(self.gain[i])
             y[rows] += g * ((x[rows] @ a.T) @ b.T)
             L[rows] += abs(g) * ((x[rows].abs() @ a.abs().T) @ b.abs().T)
-        return y, S, L
+        return y, (S, C), L
 
-    def tolerance(self, torch, y, S, L):
+    def tolerance(self, torch, y, SC, L):
+        S, C = SC
         step = torch.finfo(self.dt).eps / 2
-        tol = step * y.abs() + (3 * self.K / 16 + 8) * 2.0 ** -23 * (S + L) + self.rank * 2.0 ** -23 * L + 1e-30
+        tol = (step * y.abs() + (self.K / 8 + self.K / 256 + 16) * 2.0 ** -23 * (S + L) + self.rank * 2.0 ** -23 * L
+               + 1e-30)
         if self.dt != torch.float32:
-            tol = tol + 2.0 ** -12 * S + 2.0 ** -15 * L
+            tol = tol + 2.0 ** -11 * C + 2.0 ** -15 * L
         return tol
 
     def check(self, torch, ctx, lora=True):
