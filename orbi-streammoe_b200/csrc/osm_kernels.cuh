@@ -476,14 +476,20 @@ struct LoraArgs {
   unsigned char* planes;    // x as matrix operands [tile][K / 64][plane][NT][128 bytes]
   int* ex;                  // [tokens] exponent of each row
   int* ew;                  // [N] of each row of W
+  // the adapters of each tile of NT tokens, as prep_list describes them
+  int2* gran;               // [tile][gran_stride]
+  size_t gran_stride;
+  int2* tok;                // [tokens]
+  int* n_gran;              // [tile]
   uint32_t* wbias;          // biases as operands [N / 128][stage][32][128]
   float* v;                 // gain A x: [tokens][v_stride], or bf16 [tokens][v_planes][v_stride]
   size_t v_stride;
   int v_planes;             // 0: fp32
   int NT, split;            // tokens per tile, CTAs per tile
-  // the prep kernel: blocks for v (tiles of v_tile tokens, v_slots blocks per
-  // tile for its adapters), for W, and threads per row of x
-  int v_blocks, v_tile, v_slots, w_blocks, row_threads;
+  // the prep kernel: blocks for v (tiles of 16 tokens, v_slots blocks per tile
+  // for its adapters), for the lists, for W, and threads per row of x; after_v:
+  // blocks of the kernel that computes v instead (tiles of 32)
+  int v_blocks, v_slots, l_blocks, w_blocks, row_threads, after_v;
   int x_vec, w_vec, m_vec, a_vec, b_vec;  // 16-byte aligned rows (m: scales and biases)
 };
 cudaError_t init_lora_attributes(int max_smem);

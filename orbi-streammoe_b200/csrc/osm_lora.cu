@@ -123,9 +123,31 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// the same for pairs of 16-bit values, 16 of K
+template <int TYPE>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+  if constexpr (TYPE == 1) {
+    mma_bf16_16816(d, a0, a1, a2, a3, b0, b1);
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+// per half, the larger of m and |x| (a NaN in x is passed over, as by fmaxf)
+template <int TYPE>
+__device__ __forceinline__ uint32_t max16(uint32_t m, uint32_t x) {
+  uint32_t r;
+  if constexpr (TYPE == 1) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(x & 0x7FFF7FFFu));
+  else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(x & 0x7FFF7FFFu));
+  return r;
+}
+
 constexpr int kPrepWarps = 16;
 constexpr int kPrepThreads = kPrepWarps * 32;
-constexpr int kVCols = 32;   // rows of A per pass
+constexpr int kVCols = 32;   // rows of A per pass of prep_v
+constexpr size_t kPrepRed = (size_t)kPrepWarps * 16 * kVCols * 4;   // its partial sums
 
 // 8 consecutive values as loaded: two words of four bytes per value pair for
 // fp32, one for 16-bit types
@@ -165,113 +187,333 @@ __device__ __forceinline__ void raw_pair(const Raw8<TYPE>& r, int s, float& a, f
   }
 }
 
-// One tile of 16 MT tokens: v for the tile's distinct adapters slot, slot +
-// v_slots, ...  MT = 1: 16 warps split K; MT = 2: 8, so that a prompt's tokens
-// share the rows of A twice over.  v goes out in fp32 (few tokens) or as the
-// bf16 planes of the matrix kernel, [token][plane][v_stride].
-template <int XT, int AT, int MT>
-__device__ __forceinline__ void prep_v(const LoraArgs& a, int block, float* red) {
-  constexpr int TOK = 16 * MT, KW = kPrepWarps / MT;
-  __shared__ alignas(16) int s_id[TOK];
-  __shared__ int s_rank[TOK], s_list[TOK], s_n;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int slot = block % a.v_slots;
-  const long long t0 = (long long)(block / a.v_slots) * TOK;
-  if (warp == 0) {
+// What the blocks for v share: the tile's adapters and, for the matrix kernel,
+// the largest magnitude of each row per warp.
+struct VShared {
+  int id[32], rank[32], list[32], n;
+  float max[kPrepWarps][16];
+};
+
+// The adapters of TOK tokens from t0 on: each token's, and the first token of
+// each distinct one.  All threads.
+template <int TOK>
+__device__ __forceinline__ void list_adapters(const LoraArgs& a, long long t0, VShared& S) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  if (tid < TOK) {
     int rank = 0, id = -1;
-    if (lane < TOK && t0 + lane < a.tokens) id = adapter_of(a, t0 + lane, rank);
-    if (lane < TOK) {
-      s_id[lane] = id;
-      s_rank[lane] = rank;
-    }
-    const uint32_t same = __match_any_sync(kAllLanes, id);
-    const bool first = lane < TOK && rank > 0 && (int)__ffs(same) - 1 == lane;
-    const uint32_t firsts = __ballot_sync(kAllLanes, first);
-    if (first) s_list[__popc(firsts & ((1u << lane) - 1u))] = lane;
-    if (lane == 0) s_n = __popc(firsts);
+    if (t0 + tid < a.tokens) id = adapter_of(a, t0 + tid, rank);
+    S.id[tid] = id;
+    S.rank[tid] = rank;
   }
   __syncthreads();
-  const int g = lane >> 2, q = lane & 3, mi = warp % MT, kw = warp / MT;
-  const int r0 = mi * 16 + g;
-  for (int d = slot; d < s_n; d += a.v_slots) {
-    const int id = s_id[s_list[d]], rank = s_rank[s_list[d]];
+  if (tid < 32) {
+    int base = 0;
+    for (int b = 0; b < TOK; b += 32) {
+      const int i = b + lane;
+      bool first = i < TOK && S.rank[i < TOK ? i : 0] > 0;
+      const int mine = i < TOK ? S.id[i] : -1;
+#pragma unroll 8
+      for (int j = 0; j < b + 32 && j < TOK; ++j) first = first && !(j < i && S.id[j] == mine);
+      const uint32_t firsts = __ballot_sync(kAllLanes, first);
+      if (first) S.list[base + __popc(firsts & ((1u << lane) - 1u))] = i;
+      base += __popc(firsts);
+    }
+    if (lane == 0) S.n = base;
+  }
+  __syncthreads();
+}
+
+// v of one token and two neighbouring columns, as bf16 planes of v 2^-ex.
+__device__ __forceinline__ void store_planes(const LoraArgs& a, long long t, int j, float v0, float v1, int ex) {
+  const float sc = pow2(-ex);
+  v0 *= sc;
+  v1 *= sc;
+  uint16_t* at = reinterpret_cast<uint16_t*>(a.v) + (size_t)t * a.v_planes * a.v_stride + j;
+  for (int p = 0; p < a.v_planes; ++p) {
+    const uint32_t b = pack_bf2(v0, v1);
+    *reinterpret_cast<uint32_t*>(at + (size_t)p * a.v_stride) = b;
+    v0 -= bf_lo(b);
+    v1 -= bf_hi(b);
+  }
+}
+
+// Few tokens: tiles of 16, v for the tile's distinct adapters slot, slot +
+// v_slots, ...; the 16 warps split K.  v goes out in fp32 for the decode
+// kernel or as planes for the matrix kernel, [token][plane][v_stride].
+template <int XT, int AT>
+__device__ __forceinline__ void prep_v(const LoraArgs& a, int block, float* red, VShared& S) {
+  constexpr int TOK = 16, KW = kPrepWarps;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // the first adapters of all tiles first: blocks without work lie together
+  const int v_tiles = (int)((a.tokens + TOK - 1) / TOK), slot = block / v_tiles;
+  const long long t0 = (long long)(block % v_tiles) * TOK;
+  list_adapters<TOK>(a, t0, S);
+  const int g = lane >> 2, q = lane & 3;
+  for (int d = slot; d < S.n; d += a.v_slots) {
+    const int id = S.id[S.list[d]], rank = S.rank[S.list[d]];
     const float gain = a.gain ? a.gain[id] : 1.0f;
-    const bool in0 = s_id[r0] == id, in1 = s_id[r0 + 8] == id;
-    const bool any = __any_sync(kAllLanes, in0 || in1);
-    const size_t x0 = (size_t)(t0 + r0) * a.x_stride, x1 = (size_t)(t0 + r0 + 8) * a.x_stride;
+    const bool in0 = S.id[g] == id, in1 = S.id[g + 8] == id;
+    const size_t x0 = (size_t)(t0 + g) * a.x_stride, x1 = (size_t)(t0 + g + 8) * a.x_stride;
     const size_t arow = (size_t)id * a.a_stride;
     for (int j0 = 0; j0 < rank; j0 += kVCols) {
       float acc[kVCols / 8][4] = {};
+      float m0 = 0.0f, m1 = 0.0f;
       // K in steps of 32: the thread's 8 values of a row are the k and k + 4
       // positions of four 8-wide matrix steps (the order of K is free as long
       // as both operands use the same one)
-      if (any) {
 #pragma unroll 2
-        for (int c = kw; c < a.K / 32; c += KW) {
-          const int i = c * 32 + q * 8;
-          Raw8<XT> xa{}, xb{};
-          Raw8<AT> w[kVCols / 8] = {};
-          if (in0) xa = load_raw8<XT>(a.x, x0 + i, a.x_vec);
-          if (in1) xb = load_raw8<XT>(a.x, x1 + i, a.x_vec);
+      for (int c = warp; c < a.K / 32; c += KW) {
+        const int i = c * 32 + q * 8;
+        Raw8<XT> xa{}, xb{};
+        Raw8<AT> w[kVCols / 8] = {};
+        if (in0) xa = load_raw8<XT>(a.x, x0 + i, a.x_vec);
+        if (in1) xb = load_raw8<XT>(a.x, x1 + i, a.x_vec);
 #pragma unroll
-          for (int n = 0; n < kVCols / 8; ++n) {
-            const int j = j0 + n * 8 + g;
-            if (j < rank) w[n] = load_raw8<AT>(a.a, arow + (size_t)j * a.K + i, a.a_vec);
+        for (int n = 0; n < kVCols / 8; ++n) {
+          const int j = j0 + n * 8 + g;
+          if (j < rank) w[n] = load_raw8<AT>(a.a, arow + (size_t)j * a.K + i, a.a_vec);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          float f[4];
+          raw_pair<XT>(xa, s, f[0], f[2]);
+          raw_pair<XT>(xb, s, f[1], f[3]);
+          m0 = fmaxf(m0, fmaxf(fabsf(f[0]), fabsf(f[2])));
+          m1 = fmaxf(m1, fmaxf(fabsf(f[1]), fabsf(f[3])));
+          uint32_t h[4], l[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            h[e] = __float_as_uint(f[e]);
+            if constexpr (XT == 0) {
+              h[e] &= 0xFFFFE000u;
+              l[e] = __float_as_uint(f[e] - __uint_as_float(h[e]));
+            }
           }
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            float f[4];
-            raw_pair<XT>(xa, s, f[0], f[2]);
-            raw_pair<XT>(xb, s, f[1], f[3]);
-            uint32_t h[4], l[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              h[e] = __float_as_uint(f[e]);
-              if constexpr (XT == 0) {
-                h[e] &= 0xFFFFE000u;
-                l[e] = __float_as_uint(f[e] - __uint_as_float(h[e]));
-              }
-            }
-#pragma unroll
-            for (int n = 0; n < kVCols / 8; ++n) {
-              if (j0 + n * 8 >= rank) continue;
-              float b0, b1;
-              raw_pair<AT>(w[n], s, b0, b1);
-              if constexpr (XT == 0)
-                mma_tf32(acc[n], l[0], l[1], l[2], l[3], __float_as_uint(b0), __float_as_uint(b1));
-              mma_tf32(acc[n], h[0], h[1], h[2], h[3], __float_as_uint(b0), __float_as_uint(b1));
-            }
+          for (int n = 0; n < kVCols / 8; ++n) {
+            if (j0 + n * 8 >= rank) continue;
+            float b0, b1;
+            raw_pair<AT>(w[n], s, b0, b1);
+            if constexpr (XT == 0)
+              mma_tf32(acc[n], l[0], l[1], l[2], l[3], __float_as_uint(b0), __float_as_uint(b1));
+            mma_tf32(acc[n], h[0], h[1], h[2], h[3], __float_as_uint(b0), __float_as_uint(b1));
           }
         }
       }
+      m0 = fmaxf(m0, __shfl_xor_sync(kAllLanes, m0, 1));
+      m0 = fmaxf(m0, __shfl_xor_sync(kAllLanes, m0, 2));
+      m1 = fmaxf(m1, __shfl_xor_sync(kAllLanes, m1, 1));
+      m1 = fmaxf(m1, __shfl_xor_sync(kAllLanes, m1, 2));
+      if (q == 0) {
+        S.max[warp][g] = m0;
+        S.max[warp][g + 8] = m1;
+      }
 #pragma unroll
       for (int n = 0; n < kVCols / 8; ++n) {
-        float* at = red + ((size_t)kw * TOK + r0) * kVCols + n * 8 + 2 * q;
+        float* at = red + ((size_t)warp * TOK + g) * kVCols + n * 8 + 2 * q;
         *reinterpret_cast<float2*>(at) = make_float2(acc[n][0], acc[n][1]);
         *reinterpret_cast<float2*>(at + 8 * kVCols) = make_float2(acc[n][2], acc[n][3]);
       }
       __syncthreads();
-      for (int o = tid; o < TOK * kVCols; o += kPrepThreads) {
-        const int r = o / kVCols, j = o % kVCols;
-        float s = 0.0f;
+      if (tid < TOK * kVCols / 2) {
+        const int r = tid / (kVCols / 2), j = tid % (kVCols / 2) * 2;
+        float2 s = make_float2(0.0f, 0.0f);
+        float m = 0.0f;
 #pragma unroll
-        for (int w = 0; w < KW; ++w) s += red[((size_t)w * TOK + r) * kVCols + j];
+        for (int w = 0; w < KW; ++w) {
+          const float2 p = *reinterpret_cast<const float2*>(red + ((size_t)w * TOK + r) * kVCols + j);
+          s.x += p.x;
+          s.y += p.y;
+          m = fmaxf(m, S.max[w][r]);
+        }
         // whole pieces of 16: zeros behind the adapter's rank
-        if (s_id[r] == id && j0 + j < ((rank + 15) & ~15)) {
-          s = j0 + j < rank ? gain * s : 0.0f;
-          if (a.v_planes == 0) {
-            a.v[(size_t)(t0 + r) * a.v_stride + j0 + j] = s;
+        if (S.id[r] == id && j0 + j < ((rank + 15) & ~15)) {
+          s.x = j0 + j < rank ? gain * s.x : 0.0f;
+          s.y = j0 + j + 1 < rank ? gain * s.y : 0.0f;
+          if (a.v_planes == 0)
+            *reinterpret_cast<float2*>(a.v + (size_t)(t0 + r) * a.v_stride + j0 + j) = s;
+          else
+            store_planes(a, t0 + r, j0 + j, s.x, s.y, row_exponent(m));
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Many tokens: tiles of 32, so that a prompt's tokens share the rows of A; K in
+// stages of 64 through shared memory (rows of x and A as they are, padded so
+// that a warp's 16-byte reads meet all banks), 2 x 2 warps of 16 tokens by 32
+// rows of A.  Rows of other adapters are not loaded: they mean nothing in x's
+// part and their sums are not stored.  Bound by the matrix steps (8 clocks each
+// per quarter of an SM) for fp32 rows, by the reads of x for the others.
+template <int XT>
+struct VBig {
+  static constexpr int TOK = 32, COLS = 64, STAGES = 4, THREADS = 128;
+  static constexpr int XPITCH = XT == 0 ? 272 : 192, APITCH = 192;   // bytes
+  static constexpr size_t STAGE = (size_t)TOK * XPITCH + (size_t)COLS * APITCH;
+  static constexpr size_t BYTES = STAGES * STAGE;
+};
+template <int XT, int AT>
+__global__ void __launch_bounds__(VBig<XT>::THREADS) lora_v_kernel(const __grid_constant__ LoraArgs a) {
+  extern __shared__ uint4 v_smem[];
+  __shared__ VShared S;
+  unsigned char* const sm = reinterpret_cast<unsigned char*>(v_smem);
+  const int block = (int)blockIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  using B = VBig<XT>;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int v_tiles = (int)((a.tokens + B::TOK - 1) / B::TOK), slot = block / v_tiles;   // as in prep_v
+  const long long t0 = (long long)(block % v_tiles) * B::TOK;
+  list_adapters<B::TOK>(a, t0, S);
+  const int g = lane >> 2, q = lane & 3, wm = warp & 1, wn = warp >> 1;
+  const int r0 = wm * 16 + g, steps = a.K / 64;
+  constexpr int XB = XT == 0 ? 4 : 2, XU = XT == 0 ? 16 : 8;   // bytes of a value, 16-byte pieces of a row's stage
+  constexpr int NX = B::TOK * XU / B::THREADS, NA = B::COLS * 8 / B::THREADS;   // pieces per thread and stage
+  auto copy16 = [&](unsigned char* to, const unsigned char* from, bool vec, int align) {
+    if (vec) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to)), "l"(from) : "memory");
+    } else if (align == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        reinterpret_cast<uint32_t*>(to)[e] = reinterpret_cast<const uint32_t*>(from)[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(from)[e];
+    }
+  };
+  for (int d = slot; d < S.n; d += a.v_slots) {
+    const int id = S.id[S.list[d]], rank = S.rank[S.list[d]];
+    const float gain = a.gain ? a.gain[id] : 1.0f;
+    const bool in0 = S.id[r0] == id, in1 = S.id[r0 + 8] == id;
+    for (int j0 = 0; j0 < rank; j0 += B::COLS) {
+      const bool work = __any_sync(kAllLanes, in0 || in1) && j0 + wn * 32 < rank;
+      // this thread's pieces of a stage, null where there is nothing to load
+      const unsigned char *px[NX], *pa[NA];
+#pragma unroll
+      for (int e = 0; e < NX; ++e) {
+        const int i = tid + e * B::THREADS, r = i / XU, u = i % XU;
+        px[e] = S.id[r] == id
+                    ? static_cast<const unsigned char*>(a.x) + (size_t)(t0 + r) * a.x_stride * XB + u * 16 : nullptr;
+      }
+#pragma unroll
+      for (int e = 0; e < NA; ++e) {
+        const int i = tid + e * B::THREADS, r = i >> 3, u = i & 7;
+        pa[e] = j0 + r < rank ? static_cast<const unsigned char*>(a.a) +
+                                    ((size_t)id * a.a_stride + (size_t)(j0 + r) * a.K) * 2 + u * 16 : nullptr;
+      }
+      auto load = [&](int st) {
+        if (st < steps) {
+          unsigned char* sx = sm + (size_t)(st % B::STAGES) * B::STAGE;
+          unsigned char* sa = sx + (size_t)B::TOK * B::XPITCH;
+#pragma unroll
+          for (int e = 0; e < NX; ++e) {
+            const int i = tid + e * B::THREADS;
+            if (px[e]) {
+              copy16(sx + (i / XU) * B::XPITCH + (i % XU) * 16, px[e], a.x_vec, XB);
+              px[e] += 64 * XB;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < NA; ++e) {
+            const int i = tid + e * B::THREADS;
+            if (pa[e]) {
+              copy16(sa + (i >> 3) * B::APITCH + (i & 7) * 16, pa[e], a.a_vec, 2);
+              pa[e] += 128;
+            }
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      float acc[4][4] = {};
+      float m0 = 0.0f, m1 = 0.0f;
+      uint32_t p0 = 0, p1 = 0;               // the same as pairs of 16-bit values
+      for (int st = 0; st < B::STAGES - 1; ++st) load(st);
+      for (int st = 0; st < steps; ++st) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(B::STAGES - 2) : "memory");
+        __syncthreads();   // stage st is here, and stage st - 1 has been read by all
+        load(st + B::STAGES - 1);
+        if (!work) continue;
+        const unsigned char* sx = sm + (size_t)(st % B::STAGES) * B::STAGE;
+        const unsigned char* sa = sx + (size_t)B::TOK * B::XPITCH;
+#pragma unroll
+        for (int h2 = 0; h2 < 2; ++h2) {   // 32 of K: this thread's 8 as in prep_v
+          const int i = h2 * 32 + q * 8;
+          const Raw8<XT> xa = load_raw8<XT>(sx + r0 * B::XPITCH, i, true);
+          const Raw8<XT> xb = load_raw8<XT>(sx + (r0 + 8) * B::XPITCH, i, true);
+          Raw8<AT> w[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) w[n] = load_raw8<AT>(sa + (wn * 32 + n * 8 + g) * B::APITCH, i, true);
+          if constexpr (XT == AT) {
+            // one type: its own matrix steps of 16, exact products all the same
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              p0 = max16<XT>(p0, xa.w[e]);
+              p1 = max16<XT>(p1, xb.w[e]);
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+                if (j0 + wn * 32 + n * 8 < rank)
+                  mma16<XT>(acc[n], xa.w[2 * s], xb.w[2 * s], xa.w[2 * s + 1], xb.w[2 * s + 1], w[n].w[2 * s],
+                            w[n].w[2 * s + 1]);
           } else {
-            uint16_t* at = reinterpret_cast<uint16_t*>(a.v) + (size_t)(t0 + r) * a.v_planes * a.v_stride + j0 + j;
-            for (int p = 0; p < a.v_planes; ++p) {
-              const uint32_t b = pack_bf2(s, 0.0f) & 0xFFFFu;
-              at[(size_t)p * a.v_stride] = (uint16_t)b;
-              s -= bf_lo(b);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              float f[4];
+              raw_pair<XT>(xa, s, f[0], f[2]);
+              raw_pair<XT>(xb, s, f[1], f[3]);
+              m0 = fmaxf(m0, fmaxf(fabsf(f[0]), fabsf(f[2])));
+              m1 = fmaxf(m1, fmaxf(fabsf(f[1]), fabsf(f[3])));
+              uint32_t h[4], l[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                h[e] = __float_as_uint(f[e]);
+                if constexpr (XT == 0) {
+                  h[e] &= 0xFFFFE000u;
+                  l[e] = __float_as_uint(f[e] - __uint_as_float(h[e]));
+                }
+              }
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                if (j0 + wn * 32 + n * 8 >= rank) continue;
+                float b0, b1;
+                raw_pair<AT>(w[n], s, b0, b1);
+                if constexpr (XT == 0)
+                  mma_tf32(acc[n], l[0], l[1], l[2], l[3], __float_as_uint(b0), __float_as_uint(b1));
+                mma_tf32(acc[n], h[0], h[1], h[2], h[3], __float_as_uint(b0), __float_as_uint(b1));
+              }
             }
           }
         }
       }
-      __syncthreads();
+      if constexpr (XT == AT) {
+        float lo, hi;
+        unpack2<XT>(p0, lo, hi);
+        m0 = fmaxf(lo, hi);
+        unpack2<XT>(p1, lo, hi);
+        m1 = fmaxf(lo, hi);
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncthreads();   // all stages read before the next adapter's loads
+      if (!work) continue;
+      m0 = fmaxf(m0, __shfl_xor_sync(kAllLanes, m0, 1));
+      m0 = fmaxf(m0, __shfl_xor_sync(kAllLanes, m0, 2));
+      m1 = fmaxf(m1, __shfl_xor_sync(kAllLanes, m1, 1));
+      m1 = fmaxf(m1, __shfl_xor_sync(kAllLanes, m1, 2));
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int j = j0 + wn * 32 + n * 8 + 2 * q;
+        if (j >= ((rank + 15) & ~15)) continue;   // whole pieces of 16: zeros behind the adapter's rank
+        const bool c0 = j < rank, c1 = j + 1 < rank;
+        if (in0)
+          store_planes(a, t0 + r0, j, c0 ? gain * acc[n][0] : 0.0f, c1 ? gain * acc[n][1] : 0.0f, row_exponent(m0));
+        if (in1)
+          store_planes(a, t0 + r0 + 8, j, c0 ? gain * acc[n][2] : 0.0f, c1 ? gain * acc[n][3] : 0.0f, row_exponent(m1));
+      }
     }
   }
 }
@@ -437,29 +679,82 @@ __device__ __forceinline__ void prep_weights(const LoraArgs& a, int tile) {
   }
 }
 
-// First the blocks for v, then those for W, then rows of x, up to the next
-// multiple of 16 (zero rows behind the last).
+// The adapters of one tile of the matrix kernel: pieces of 16 rows of each, in
+// the order of their first tokens, {adapter, first row | rows from there << 16};
+// and each token's first piece and number of pieces (0: no adapter).
+__device__ __forceinline__ void prep_list(const LoraArgs& a, int tile) {
+  constexpr int kMost = 256;               // tokens of a tile
+  __shared__ alignas(16) int s_id[kMost];
+  __shared__ int s_goff[kMost], s_sum[kMost / 32];
+  const int n = threadIdx.x, lane = n & 31;
+  const long long t = (long long)tile * a.NT + n;
+  int rank = 0, id = -1;
+  if (n < a.NT && t < a.tokens) id = adapter_of(a, t, rank);
+  if (rank == 0) id = -1;
+  if (n < kMost) s_id[n] = id;
+  __syncthreads();
+  int first = n;
+  if (id >= 0) {
+    const int4* ids4 = reinterpret_cast<const int4*>(s_id);
+    for (int j = 0; j * 4 < n; ++j) {
+      const int4 v = ids4[j];
+      const int f = v.x == id ? 0 : v.y == id ? 1 : v.z == id ? 2 : v.w == id ? 3 : 4;
+      if (f < 4) {
+        first = min(first, j * 4 + f);
+        break;
+      }
+    }
+  }
+  const int pieces = id >= 0 ? (rank + 15) >> 4 : 0, mine = first == n ? pieces : 0;
+  int incl = mine;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const int up = __shfl_up_sync(kAllLanes, incl, s);
+    if (lane >= s) incl += up;
+  }
+  if (n < kMost && lane == 31) s_sum[n >> 5] = incl;
+  __syncthreads();
+  int base = 0, all = 0;
+  for (int w = 0; w < kMost / 32; ++w) {
+    if (w < (n >> 5)) base += s_sum[w];
+    all += s_sum[w];
+  }
+  const int goff = base + incl - mine;
+  if (n < kMost) s_goff[n] = goff;
+  __syncthreads();
+  int2* gran = a.gran + (size_t)tile * a.gran_stride;
+  for (int i = 0; i < mine; ++i) gran[goff + i] = make_int2(id, i * 16 | (rank - i * 16) << 16);
+  if (n < a.NT && t < (a.tokens + 15) / 16 * 16) a.tok[t] = make_int2(id >= 0 ? s_goff[first] : 0, pieces);
+  if (n == 0) a.n_gran[tile] = all;
+}
+
+// First the blocks for v, then the tiles' lists, then those for W, then rows of
+// x, up to the next multiple of 16 (zero rows behind the last).
 template <int XT, int AT>
 __global__ void __launch_bounds__(kPrepThreads, 2) lora_prep_kernel(const __grid_constant__ LoraArgs a) {
-  __shared__ alignas(16) float s_red[kPrepWarps * 16 * kVCols];
-  pdl_wait();
+  extern __shared__ uint4 prep_smem[];     // the partial sums of prep_v
+  __shared__ VShared s_v;
+  // behind lora_v_kernel this one does not wait for it to begin: that kernel has
+  // waited for everything before it, and neither reads what the other writes
+  if (!a.after_v) pdl_wait();
   pdl_trigger();
-  if ((int)blockIdx.x < a.v_blocks) {
-    if (a.v_tile == 16) prep_v<XT, AT, 1>(a, (int)blockIdx.x, s_red);
-    else prep_v<XT, AT, 2>(a, (int)blockIdx.x, s_red);
-    return;
-  }
-  if ((int)blockIdx.x < a.v_blocks + a.w_blocks) {
-    prep_weights<XT == 0>(a, (int)blockIdx.x - a.v_blocks);
-    return;
-  }
-  const long long b = (long long)blockIdx.x - a.v_blocks - a.w_blocks;
-  if (a.row_threads == kPrepThreads) {
-    prep_row<XT, kPrepThreads>(a, b);
+  long long b = blockIdx.x;
+  if (b < a.v_blocks) {
+    prep_v<XT, AT>(a, (int)b, reinterpret_cast<float*>(prep_smem), s_v);
+  } else if ((b -= a.v_blocks) < a.l_blocks) {
+    prep_list(a, (int)b);
+  } else if ((b -= a.l_blocks) < a.w_blocks) {
+    prep_weights<XT == 0>(a, (int)b);
   } else {
-    const long long t = b * kPrepWarps + (threadIdx.x >> 5);
-    if (t < (a.tokens + 15) / 16 * 16) prep_row<XT, 32>(a, t);
+    b -= a.w_blocks;
+    if (a.row_threads == kPrepThreads) {
+      prep_row<XT, kPrepThreads>(a, b);
+    } else {
+      const long long t = b * kPrepWarps + (threadIdx.x >> 5);
+      if (t < (a.tokens + 15) / 16 * 16) prep_row<XT, 32>(a, t);
+    }
   }
+  if (a.after_v) pdl_wait();               // who waits for this kernel has v too
 }
 
 // ---------------------------------------------------------------- few tokens
@@ -563,7 +858,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) lora_decode_kernel(const __gri
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       for (int j = lane; j < rank[t]; j += 32) {
-        const float v = a.v[(size_t)t * a.v_stride + j];
+        const float v = __ldcg(a.v + (size_t)t * a.v_stride + j);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
           const float bv = j == lane ? b[r][t]
@@ -587,20 +882,26 @@ __global__ void __launch_bounds__(kDecWarps * 32) lora_decode_kernel(const __gri
 
 // ---------------------------------------------------------------- gemm
 
+// What the prep kernel wrote is read with __ldcg: this kernel starts beside
+// that one, so lines of an earlier call could still be in L1.
+
 constexpr int kLgM = 128;                 // rows of W per tile
 constexpr int kLgConv = 8;                // converter warps, two groups of four
 constexpr int kLgEpi = 8;                 // epilogue warps, two per quarter of the rows
-constexpr int kLgWarps = 2 + kLgConv + kLgEpi;
-constexpr int kLgThreads = kLgWarps * 32;
-constexpr int kLgMaxN = 256;
-constexpr int kLgGran = kLgMaxN * 8;      // 16-wide pieces of adapters: 256 tokens of rank 128
+constexpr int kLgThreads = (2 + kLgConv + kLgEpi) * 32;
 constexpr int kLgRO = 4;                  // operand stages (one K group each)
-constexpr int kLgRQ = 4;                  // Q4 tiles (32 rows of one K group) in flight per converter warp
+constexpr int kLgRQ = 2;                  // Q4 tiles (32 rows of one K group) in flight per converter warp
 constexpr int kLgQPitch = 48;             // bytes per row of a Q4 tile: 16-byte reads of 8 rows meet all banks
-constexpr size_t kLgStage = 32768;        // x: 256 tokens of one plane or 128 of two
+constexpr size_t kLgA = 16384;            // W's part of a stage, 128 rows of 64 fp16
+constexpr size_t kLgX = 32768;            // x's part: 256 tokens of one plane or 128 of two
+constexpr size_t kLgStage = kLgA + kLgX;
 constexpr size_t kLgQTile = (size_t)32 * kLgQPitch;
-constexpr uint32_t kLgTmemA = 256;        // below: two sums of 128 tokens or one of 256
 
+// Both operands are in shared memory.  With the converted weights in tensor
+// memory instead, stores to it bound the kernel at about 0.6 us per 128 x 64
+// weights, however many warps convert.  What is left for tensor memory are two
+// buffers of 256 tokens' sums, so that a tile's epilogue runs beside the next
+// tile's products.
 template <bool F32>
 struct LgCfg {
   static constexpr int PL = F32 ? 2 : 1;        // planes of x
@@ -608,24 +909,18 @@ struct LgCfg {
   static constexpr int GROUP = F32 ? 4 : 1 << 30;  // stages per partial sum
   static constexpr int NV = F32 ? 3 : 2;        // bf16 planes of v
 };
-// Per-tile lists, two buffers: written by the epilogue warps for all roles.
-struct alignas(16) LgList {
-  int id[kLgMaxN];          // adapter of each token, -1 none
-  float fx[kLgMaxN];        // 2^exponent of the tokens' rows
-  uint16_t first[kLgMaxN];  // first token of the tile with the same adapter, 0xFFFF none
-  uint16_t rank[kLgMaxN];
-  uint16_t goff[kLgMaxN];   // first piece of the adapter, at its first token
-  uint16_t gran[kLgGran];   // piece: first token << 4 | index of the 16 rows
-  int n_gran;
-  int wsum[kLgEpi];
+// A converter warp's first block of adapters in a tile, brought ahead: the
+// pieces, and the entries of its threads' tokens.
+struct alignas(16) LgAhead {
+  int2 gran[4], tok[2][32];
 };
 struct LgShared {
-  LgList list[2];
+  LgAhead ahead[kLgConv];
   int ew[kLgM];             // exponents of the tile's rows of W
   int bad;                  // some B held a non-finite value
   volatile int abort;
   uint32_t tmem;
-  uint64_t opfull[kLgRO], opempty[kLgRO], accfull[2], accempty[2], listfull[2], epi;
+  uint64_t opfull[kLgRO], opempty[kLgRO], accfull[2], accempty[2];
 };
 constexpr size_t kLgSmem = kLgRO * kLgStage + kLgConv * kLgRQ * kLgQTile + sizeof(LgShared) + 1024;
 
@@ -652,7 +947,6 @@ __device__ __forceinline__ int ld_cluster_i(uint32_t addr) {
   asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
@@ -670,7 +964,9 @@ __device__ __forceinline__ uint4 load_meta(const LoraArgs& a, const uint16_t* ba
 // Adds to y[t][o] the terms of B's values that are not finite (their places in
 // the matrix product were taken as zero).
 template <int XT, int AT>
-__device__ __noinline__ void add_bad_terms(const LoraArgs& a, int id, int rank, int o, long long t) {
+__device__ __noinline__ void add_bad_terms(const LoraArgs& a, int o, long long t) {
+  int rank;
+  const int id = adapter_of(a, t, rank);
   float s = 0.0f;
   bool any = false;
   for (int j = 0; j < rank; ++j) {
@@ -678,8 +974,9 @@ __device__ __noinline__ void add_bad_terms(const LoraArgs& a, int id, int rank, 
     if (!isfinite(w)) {
       float v = 0.0f;
       for (int p = a.v_planes - 1; p >= 0; --p)
-        v += bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.v)[((size_t)t * a.v_planes + p) * a.v_stride + j]);
-      s += w * v;
+        v += bf16_bits_to_f32(__ldcg(reinterpret_cast<const uint16_t*>(a.v) +
+                                     ((size_t)t * a.v_planes + p) * a.v_stride + j));
+      s += w * (v * pow2(__ldcg(a.ex + t)));   // the planes hold v 2^-ex
       any = true;
     }
   }
@@ -687,18 +984,52 @@ __device__ __noinline__ void add_bad_terms(const LoraArgs& a, int id, int rank, 
   if (any) store_val<XT>(a.y, at, load_val<XT>(a.y, at) + s);
 }
 
+// Bounded wait on an mbarrier phase: after about two seconds (4e9 clocks) the
+// status bit is set and the CTA-wide abort flag makes all later waits return.
+// It counts clocks, not the global timer, whose read takes long enough to show
+// on every wait that does not succeed at once.
+__device__ __forceinline__ bool lg_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t* status) {
+  if (mbar_try_sleep(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_sleep(bar, parity)) return true;
+    if (*abort) return false;
+    if (clock64() - t0 > 4000000000ll) break;
+  }
+  *abort = 1;
+  atomicOr(status, kStatusCopyTimeout);
+  return false;
+}
+// By a whole warp, with one outcome for all its lanes.
+__device__ __forceinline__ bool lg_warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t* status) {
+  return __all_sync(kAllLanes, lg_wait(bar, parity, abort, status));
+}
+
+// D[tmem] (+)= A[smem desc] * B[smem desc]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(ad), "l"(bd), "r"(idesc), "r"(acc));
+}
+
+// Warp 0 brings x, warp 1 issues the matrix steps, 8 warps convert weights and
+// adapters (two groups, every other stage each), 8 warps read the sums (fp32
+// rows after every four stages) and write y.
 template <int XT, int AT>
 __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_constant__ LoraArgs a) {
   constexpr bool F32 = XT == 0;
   using C = LgCfg<F32>;
-  constexpr int PL = C::PL;
+  constexpr int PL = C::PL, M = kLgM;
   extern __shared__ unsigned char lg_raw[];
   unsigned char* stages = lg_raw + ((1024u - (smem_addr(lg_raw) & 1023u)) & 1023u);
   unsigned char* qtiles = stages + kLgRO * kLgStage;
   LgShared& S = *reinterpret_cast<LgShared*>(qtiles + kLgConv * kLgRQ * kLgQTile);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = a.split, rank_c = split > 1 ? (int)cluster_rank() : 0;
-  const int mt = (a.N + kLgM - 1) / kLgM, nt = (int)((a.tokens + a.NT - 1) / a.NT);
+  const int mt = (a.N + M - 1) / M, nt = (int)((a.tokens + a.NT - 1) / a.NT);
   const int tiles = mt * nt;
   const int first_tile = split > 1 ? (int)blockIdx.x / split : (int)blockIdx.x;
   const int step = split > 1 ? tiles : (int)gridDim.x;  // a cluster has one tile
@@ -707,7 +1038,6 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
   const int nk = a.K >> 6, nbk = (nk + 63) >> 6, nkv = nk + (F32 ? 2 : 1) * nbk;
   const int k_lo = nkv * rank_c / split, nkm = nkv * (rank_c + 1) / split - k_lo;
   const int nq = max(0, min(nk - k_lo, nkm));   // of them from Q4 rows
-  const int nbuf = a.NT <= 128 ? 2 : 1;
   volatile int* abort = &S.abort;
   if (tid == 0) {
     for (int i = 0; i < kLgRO; ++i) {
@@ -717,9 +1047,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S.accfull[i], 1);
       mbar_init(&S.accempty[i], kLgEpi);
-      mbar_init(&S.listfull[i], kLgEpi);
     }
-    mbar_init(&S.epi, kLgEpi);
     S.bad = 0;
     S.abort = 0;
     mbar_init_fence();
@@ -733,13 +1061,16 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
   fence_after();
   const uint32_t tmem = S.tmem;
   auto tokens_of = [&](int tile) { return (int)min((long long)a.NT, a.tokens - (long long)(tile / mt) * a.NT); };
-  // planes of v that a stage holds, and the passes over the adapters that makes
+  // The adapters' stages: blocks of 64 columns, this CTA's share of them, each
+  // in passes over B's parts (fp16 adapters: hi, lo) and as many planes of v as
+  // a stage holds.
+  constexpr int BPARTS = AT == 2 ? 2 : 1;
   auto v_planes = [&](int npad) { return min(C::NV, 256 / npad); };
   auto v_passes = [&](int npad) { const int p = v_planes(npad); return (C::NV + p - 1) / p; };
-  // stages this CTA adds for the adapters of a tile (its share of the blocks of 64 columns)
-  auto lora_stages = [&](int ng, int npad) {
+  auto pieces_at = [&](int tile) { return a.adapter && tile < tiles ? __ldcg(a.n_gran + tile / mt) : 0; };
+  auto stages_of = [&](int npad, int ng) {
     const int nb = (ng + 3) >> 2;
-    return nb > rank_c ? (nb - rank_c + split - 1) / split * v_passes(npad) : 0;
+    return nkm + (nb > rank_c ? (nb - rank_c + split - 1) / split * BPARTS * v_passes(npad) : 0);
   };
 
   if (warp == 0) {
@@ -747,27 +1078,21 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
     if (lane == 0) {
       pdl_wait();
       uint32_t os = 0;
-      int ti = 0;
       bool ok = true;
-      for (int tile = first_tile; tile < tiles && ok; tile += step, ++ti) {
+      int ng = pieces_at(first_tile);
+      for (int tile = first_tile; tile < tiles && ok; tile += step) {
         const int npad = (tokens_of(tile) + 15) & ~15;
         const unsigned char* src = a.planes + (size_t)(tile / mt) * (nk + nbk) * PL * a.NT * 128;
-        int total = nkm;
+        const int total = stages_of(npad, ng);
+        ng = pieces_at(tile + step);
         for (int c = 0; c < total; ++c, ++os) {
-          if (c == nkm - 1) {
-            if (!tc_wait(&S.listfull[ti & 1], (ti >> 1) & 1, abort, a.status)) {
-              ok = false;
-              break;
-            }
-            total += lora_stages(S.list[ti & 1].n_gran, npad);
-          }
           const int st = (int)(os % kLgRO);
-          if (os >= (uint32_t)kLgRO && !tc_wait(&S.opempty[st], ((os / kLgRO) - 1) & 1, abort, a.status)) {
+          if (os >= (uint32_t)kLgRO && !lg_wait(&S.opempty[st], ((os / kLgRO) - 1) & 1, abort, a.status)) {
             ok = false;
             break;
           }
           if (c < nkm) {
-            unsigned char* dst = stages + (size_t)st * kLgStage;
+            unsigned char* dst = stages + (size_t)st * kLgStage + kLgA;
             const int k = k_lo + c, kp = k < nk ? k : nk + (F32 ? (k - nk) >> 1 : k - nk);
             mbar_arrive_expect(&S.opfull[st], (uint32_t)(PL * npad * 128));
 #pragma unroll
@@ -789,64 +1114,51 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     if (lane == 0) {
-      const uint64_t bdesc0 = desc_sw128(smem_addr(stages));
+      pdl_wait();   // the lists
+      const uint64_t adesc0 = desc_sw128(smem_addr(stages)), bdesc0 = adesc0 + (kLgA >> 4);
       uint32_t os = 0, gq = 0;
-      int ti = 0;
       bool ok = true;
-      for (int tile = first_tile; tile < tiles && ok; tile += step, ++ti) {
+      int ng = pieces_at(first_tile);
+      for (int tile = first_tile; tile < tiles && ok; tile += step) {
         const int npad = (tokens_of(tile) + 15) & ~15;
         const uint32_t idf = idesc16(kLgM, npad, false), idb = idesc16(kLgM, npad, true);
-        const int vpl = v_planes(npad), passes = v_passes(npad);
-        int total = nkm;
-        uint32_t d = 0;
+        const int vpl = v_planes(npad), vps = v_passes(npad);
+        const int total = stages_of(npad, ng);
+        ng = pieces_at(tile + step);
         for (int c = 0; c < total; ++c, ++os) {
-          if (c == nkm - 1) {
-            if (!tc_wait(&S.listfull[ti & 1], (ti >> 1) & 1, abort, a.status)) {
-              ok = false;
-              break;
-            }
-            total += lora_stages(S.list[ti & 1].n_gran, npad);
-          }
-          const int b = nbuf == 2 ? (int)(gq & 1) : 0;
           bool first = c % C::GROUP == 0;
-          if (first) {
-            const uint32_t use = nbuf == 2 ? gq >> 1 : gq;
-            if (use > 0 && !tc_wait(&S.accempty[b], (use - 1) & 1, abort, a.status)) {
-              ok = false;
-              break;
-            }
-            d = tmem + (uint32_t)(b * 128);
+          if (first && gq >= 2 && !lg_wait(&S.accempty[gq & 1], ((gq >> 1) - 1) & 1, abort, a.status)) {
+            ok = false;
+            break;
           }
+          const uint32_t d = tmem + (gq & 1) * 256;
           const int st = (int)(os % kLgRO);
-          if (!tc_wait(&S.opfull[st], (os / kLgRO) & 1, abort, a.status)) {
+          if (!lg_wait(&S.opfull[st], (os / kLgRO) & 1, abort, a.status)) {
             ok = false;
             break;
           }
           fence_after();
-          const uint32_t ab = tmem + kLgTmemA + (uint32_t)st * 64;
-          const uint64_t bd = bdesc0 + (uint64_t)st * (kLgStage >> 4);
-          auto issue = [&](int pa, uint32_t boff, uint32_t id) {
+          const uint64_t so = (uint64_t)st * (kLgStage >> 4);
+          auto issue = [&](uint32_t boff, uint32_t id) {
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-              mma_ts(d, ab + (uint32_t)(pa * 32 + ks * 8), bd + (uint64_t)((boff + ks * 32) >> 4), id,
+              mma_ss(d, adesc0 + so + (uint64_t)(ks * 2), bdesc0 + so + (uint64_t)((boff + ks * 32) >> 4), id,
                      first && ks == 0 ? 0u : 1u);
             first = false;
           };
           if (c < nkm) {
-            issue(0, 0, idf);
+            issue(0, idf);
             // the lo part of x; not for the lo part of the biases
-            if (F32 && (k_lo + c < nk || ((k_lo + c - nk) & 1) == 0)) issue(0, (uint32_t)C::NMAX * 128, idf);
+            if (F32 && (k_lo + c < nk || ((k_lo + c - nk) & 1) == 0)) issue((uint32_t)C::NMAX * 128, idf);
           } else {
-            const int p0 = (c - nkm) % passes * vpl;
-            for (int p = 0; p < vpl && p0 + p < C::NV; ++p) {
-              issue(0, (uint32_t)(p * npad * 128), idb);
-              // fp16 adapters: the lo part of B against all but the last plane of v
-              if (AT == 2 && p0 + p < C::NV - 1) issue(1, (uint32_t)(p * npad * 128), idb);
-            }
+            const int pass = (c - nkm) % (BPARTS * vps), p0 = pass % vps * vpl;
+            // the lo part of B meets all but the last plane of v
+            const int planes = min(pass >= vps ? C::NV - 1 : C::NV, p0 + vpl) - p0;
+            for (int p = 0; p < planes; ++p) issue((uint32_t)(p * npad * 128), idb);
           }
           commit(&S.opempty[st]);
           if (c % C::GROUP == C::GROUP - 1 || c == total - 1) {
-            commit(&S.accfull[b]);
+            commit(&S.accfull[gq & 1]);
             ++gq;
           }
         }
@@ -856,10 +1168,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
   } else if (warp < 2 + kLgConv) {
     // ---------------- converters: group 0 the even stages of a tile, group 1 the odd ones ----------------
     const int grp = (warp - 2) >> 2;
-    const int quad = warp & 3;
-    const int row = quad * 32 + lane;        // tensor-memory lane = row of the tile
-    const int gt = ((warp - 2) & 3) * 32 + lane;
-    const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
+    const int row = ((warp - 2) & 3) * 32 + lane;   // row of the tile
     unsigned char* ring = qtiles + (size_t)(warp - 2) * kLgRQ * kLgQTile;
     // Q4 tiles of this warp's stages, kLgRQ of them ahead: 16 bytes per lane and
     // copy, two lanes per row
@@ -869,7 +1178,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
     auto f_rows = [&]() {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int r = (f_tile % mt) * kLgM + quad * 32 + (lane >> 1) + 16 * i;
+        const int r = (f_tile % mt) * M + (row & 96) + (lane >> 1) + 16 * i;
         f_src[i] = f_tile < tiles && r < a.N
                        ? a.packed + (size_t)r * (a.K >> 3) + (size_t)(k_lo + grp) * 8 + (lane & 1) * 4 : nullptr;
       }
@@ -902,409 +1211,326 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
     for (int i = 0; i < kLgRQ; ++i) fetch();
     pdl_wait();
     uint32_t os = 0;                         // stages before this tile
-    int ti = 0;
     bool ok = true;
-    for (int tile = first_tile; tile < tiles && ok; tile += step, ++ti) {
-      const int m_tile = tile % mt, o = m_tile * kLgM + row;
+    int ng_next = pieces_at(first_tile), ew_next = __ldcg(a.ew + (first_tile % mt) * M + row);
+    for (int tile = first_tile; tile < tiles && ok; tile += step) {
+      const int o = (tile % mt) * M + row;
       const bool live = o < a.N;
-      const float wsc = pow2(-a.ew[o]);
-      const LgList& L = S.list[ti & 1];
-      const int npad = (tokens_of(tile) + 15) & ~15, vpl = v_planes(npad), passes = v_passes(npad);
-      int total = nkm, ng = 0;
-      bool listed = false;
+      const long long tn = (long long)(tile / mt) * a.NT;
+      const float wsc = pow2(-ew_next);
+      const int ntok = tokens_of(tile), npad = (ntok + 15) & ~15;
+      const int ng = ng_next, total = stages_of(npad, ng);
+      ng_next = pieces_at(tile + step);
+      if (tile + step < tiles) ew_next = __ldcg(a.ew + ((tile + step) % mt) * M + row);
       uint4 meta = make_uint4(0, 0, 0, 0), meta_n = meta;
       int m8 = -1;
       auto slot_free = [&](uint32_t oc) {
-        if (oc >= (uint32_t)kLgRO && !warp_wait(&S.opempty[oc % kLgRO], ((oc / kLgRO) - 1) & 1, abort, a.status))
-          return false;
-        fence_after();
-        return true;
+        return oc < (uint32_t)kLgRO || lg_warp_wait(&S.opempty[oc % kLgRO], ((oc / kLgRO) - 1) & 1, abort, a.status);
       };
-      for (int c = grp;; c += 2) {
-        if (c >= nkm && !listed) {
-          if (!warp_wait(&S.listfull[ti & 1], (ti >> 1) & 1, abort, a.status)) {
-            ok = false;
-            break;
-          }
-          ng = L.n_gran;
-          total = nkm + lora_stages(ng, npad);
-          listed = true;
-        }
-        if (c >= total) break;
-        const uint32_t oc = os + (uint32_t)c;
-        const int st = (int)(oc % kLgRO);
-        const uint32_t ab = tmem + lane_addr + kLgTmemA + (uint32_t)st * 64;
-        if (c < nkm) {
-          uint32_t av[32];
-          if (c < nq) {
-            const int k = k_lo + c;
-            if (live && (k >> 3) != m8) {
-              meta = m8 >= 0 && (k >> 3) == m8 + 1 ? meta_n : load_meta(a, a.scales, o, k >> 3);
-              m8 = k >> 3;
-              if ((m8 + 1) * 8 < nk) meta_n = load_meta(a, a.scales, o, m8 + 1);
-            }
-            asm volatile("cp.async.wait_group %0;" ::"n"(kLgRQ - 1) : "memory");
-            __syncwarp();                    // the other lanes' copies too
-            const unsigned char* q = ring + (used % kLgRQ) * kLgQTile + lane * kLgQPitch;
-            const uint4 w0 = *reinterpret_cast<const uint4*>(q), w1 = *reinterpret_cast<const uint4*>(q + 16);
-            ++used;
-            __syncwarp();                    // read by all lanes before the tile is filled again
-            fetch();
-            const uint32_t wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-            const uint32_t sw = word_of(meta, (k >> 1) & 3);
-            // scale (q - 8), at most 8 + 3 significant bits and so exact in fp16:
-            // a nibble in the mantissa of 16.0 is 16 + q, and 24 scale is exact too.
-            // The pairs are (q_i, q_i+4) of a word; x is laid out alike.
-            const __half2 s2 = __float2half2_rn((k & 1 ? bf_hi(sw) : bf_lo(sw)) * wsc),
-                          m24 = __hmul2(s2, __float2half2_rn(-24.0f));
-#pragma unroll
-            for (int w = 0; w < 8; ++w) {
-              const uint32_t v[4] = {wv[w] << 6, wv[w] << 2, wv[w] >> 2, wv[w] >> 6};
-#pragma unroll
-              for (int p = 0; p < 4; ++p)
-                av[4 * w + p] = h2u(__hfma2(u2h((v[p] & 0x03C003C0u) | 0x4C004C00u), s2, m24));
-            }
-          } else {
-            // the biases of 64 groups
-            const uint32_t* b = a.wbias + ((size_t)m_tile * (nkv - nk) + (size_t)(k_lo + c - nk)) * 32 * 128 + row;
-#pragma unroll
-            for (int e = 0; e < 32; ++e) av[e] = __ldg(b + e * 128);
-          }
-          if (!slot_free(oc)) {
-            ok = false;
-            break;
-          }
-          st32(ab, av);
-        } else {
-          // a block of 64 columns: four pieces of 16 rows of adapters
-          const int lc = c - nkm, blk = rank_c + lc / passes * split, p0 = lc % passes * vpl;
-          int left[4];                       // rows of the adapter from this piece on, 0: no piece
-          uint4 raw[4][2];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int gr = blk * 4 + q < ng ? (int)L.gran[blk * 4 + q] : 0xFFFF;
-            raw[q][0] = raw[q][1] = make_uint4(0, 0, 0, 0);
-            left[q] = 0;
-            if (gr != 0xFFFF && live) {
-              const int j0 = (gr & 15) * 16;
-              left[q] = (int)L.rank[gr >> 4] - j0;
-              const uint16_t* at = static_cast<const uint16_t*>(a.b) + (size_t)L.id[gr >> 4] * a.b_stride +
-                                   (size_t)o * a.rank + j0;
-              if (a.b_vec && j0 + 16 <= a.rank) {
-                raw[q][0] = __ldg(reinterpret_cast<const uint4*>(at));
-                raw[q][1] = __ldg(reinterpret_cast<const uint4*>(at) + 1);
-              } else {
-                uint32_t h[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) h[e] = e < left[q] ? at[e] : 0u;
-                raw[q][0] = make_uint4(pack2(h[0], h[1]), pack2(h[2], h[3]), pack2(h[4], h[5]), pack2(h[6], h[7]));
-                raw[q][1] =
-                    make_uint4(pack2(h[8], h[9]), pack2(h[10], h[11]), pack2(h[12], h[13]), pack2(h[14], h[15]));
-              }
-            }
-          }
-          // this thread's first token: its pieces in the block, the first one's v
-          auto pieces_of = [&](int n, int& q0, int& q1) {
-            const int mine = n < npad ? (int)L.first[n] : 0xFFFF;
-            q0 = q1 = 4;
-            if (mine != 0xFFFF) {
-              const int g0 = (int)L.goff[mine] - blk * 4, g1 = g0 + (((int)L.rank[n] + 15) >> 4);
-              q0 = max(0, min(4, g0));
-              q1 = max(0, min(4, g1));
-            }
-            return (blk * 4 - (mine != 0xFFFF ? (int)L.goff[mine] : 0)) * 16;   // column 0 of the block, in its v
-          };
-          const long long tn = (long long)(tile / mt) * a.NT;
-          int q0, q1;
-          int j0 = pieces_of(gt, q0, q1);
-          // the planes of this pass, 16 columns each
-          uint4 f[C::NV][2];
-          const uint16_t* vp = reinterpret_cast<const uint16_t*>(a.v) + (size_t)p0 * a.v_stride;
-          auto load_v = [&](int n, int j) {
-            const uint16_t* at = vp + (size_t)(tn + n) * C::NV * a.v_stride + j;
-#pragma unroll
-            for (int p = 0; p < C::NV; ++p)
-              if (p < vpl && p0 + p < C::NV) {
-                f[p][0] = *reinterpret_cast<const uint4*>(at + (size_t)p * a.v_stride);
-                f[p][1] = *reinterpret_cast<const uint4*>(at + (size_t)p * a.v_stride + 8);
-              }
-          };
-          int ex = 0;
-          if (q0 < q1) {
-            ex = a.ex[tn + gt];
-            load_v(gt, j0 + q0 * 16);
-          }
-          if (!slot_free(oc)) {
-            ok = false;
-            break;
-          }
-          // ---- B ----
-          const uint32_t wsc2 = pack_bf2(wsc, wsc);
-          __syncwarp();
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t w[8] = {raw[q][0].x, raw[q][0].y, raw[q][0].z, raw[q][0].w,
-                             raw[q][1].x, raw[q][1].y, raw[q][1].z, raw[q][1].w};
-            if (left[q] < 16) {
-#pragma unroll
-              for (int p = 0; p < 8; ++p)
-                w[p] &= (2 * p < left[q] ? 0xFFFFu : 0u) | (2 * p + 1 < left[q] ? 0xFFFF0000u : 0u);
-            }
-            // a non-finite value must not meet the zeros of other tokens: an
-            // exponent of all ones carries into the sign place
-            constexpr uint32_t kExp = AT == 2 ? 0x7C007C00u : 0x7F807F80u, kOne = AT == 2 ? 0x04000400u : 0x00800080u;
-            uint32_t any = 0;
-#pragma unroll
-            for (int p = 0; p < 8; ++p) any |= (w[p] & kExp) + kOne;
-            if (any & 0x80008000u) {
-              S.bad = 1;
-#pragma unroll
-              for (int p = 0; p < 8; ++p) {
-                const uint32_t b = ((w[p] & kExp) + kOne) & 0x80008000u;
-                w[p] &= ~((b >> 15) * 0xFFFFu);
-              }
-            }
-            __syncwarp();
-            if constexpr (AT == 2) {
-              uint32_t hi[8], lo[8];
-#pragma unroll
-              for (int p = 0; p < 8; ++p) {
-                float w0, w1;
-                unpack2<AT>(w[p], w0, w1);
-                w0 *= wsc;
-                w1 *= wsc;
-                hi[p] = pack_bf2(w0, w1);
-                lo[p] = pack_bf2(w0 - bf_lo(hi[p]), w1 - bf_hi(hi[p]));
-              }
-              st8(ab + (uint32_t)(q * 8), hi);
-              st8(ab + (uint32_t)(32 + q * 8), lo);
-            } else {
-#pragma unroll
-              for (int p = 0; p < 8; ++p) w[p] = bf2_fma(w[p], wsc2, 0x80008000u);   // a power of two: exact
-              st8(ab + (uint32_t)(q * 8), w);
-            }
-          }
-          unsigned char* dst = stages + (size_t)st * kLgStage;
-          // ---- v: zeros, and in each token's columns its own planes ----
-          for (int n = gt; n < npad; n += 128) {
-            if (n != gt) {
-              j0 = pieces_of(n, q0, q1);
-              if (q0 < q1) {
-                ex = a.ex[tn + n];
-                load_v(n, j0 + q0 * 16);
-              }
-            }
-            unsigned char* at = dst + (size_t)n * 128;
-            const uint4 zero = make_uint4(0, 0, 0, 0);
-            const float xsc = pow2(-ex);
-            const uint32_t xsc2 = pack_bf2(xsc, xsc);   // a power of two: exact
-#pragma unroll
-            for (int p = 0; p < C::NV; ++p) {
-              if (p >= vpl || p0 + p >= C::NV) continue;
-#pragma unroll
-              for (int u = 0; u < 8; ++u)
-                if ((u >> 1) < q0 || (u >> 1) >= q1)
-                  *reinterpret_cast<uint4*>(at + (size_t)p * npad * 128 + ((u ^ (n & 7)) << 4)) = zero;
-            }
-            for (int q = q0; q < q1; ++q) {
-              if (q != q0) load_v(n, j0 + q * 16);
-#pragma unroll
-              for (int p = 0; p < C::NV; ++p) {
-                if (p >= vpl || p0 + p >= C::NV) continue;
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                  *reinterpret_cast<uint4*>(at + (size_t)p * npad * 128 + (((2 * q + u) ^ (n & 7)) << 4)) =
-                      make_uint4(bf2_fma(f[p][u].x, xsc2, 0x80008000u), bf2_fma(f[p][u].y, xsc2, 0x80008000u),
-                                 bf2_fma(f[p][u].z, xsc2, 0x80008000u), bf2_fma(f[p][u].w, xsc2, 0x80008000u));
-              }
-            }
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        wait_st();
-        fence_before();
+      auto slot_done = [&](int st) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.opfull[st]);
+      };
+      // 16 bytes of this row's operand, in the 128-byte swizzle
+      auto put = [&](int st, int u, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+        *reinterpret_cast<uint4*>(stages + (size_t)st * kLgStage + row * 128 + ((u ^ (row & 7)) << 4)) =
+            make_uint4(x, y, z, w);
+      };
+      // ---- a stage of weights or biases ----
+      auto weights = [&](int c) -> bool {
+        const uint32_t oc = os + (uint32_t)c;
+        const int st = (int)(oc % kLgRO);
+        uint32_t av[32];
+        if (c < nq) {
+          const int k = k_lo + c;
+          if (live && (k >> 3) != m8) {
+            meta = m8 >= 0 && (k >> 3) == m8 + 1 ? meta_n : load_meta(a, a.scales, o, k >> 3);
+            m8 = k >> 3;
+            if ((m8 + 1) * 8 < nk) meta_n = load_meta(a, a.scales, o, m8 + 1);
+          }
+          asm volatile("cp.async.wait_group %0;" ::"n"(kLgRQ - 1) : "memory");
+          __syncwarp();                      // the other lanes' copies too
+          const unsigned char* q = ring + (used % kLgRQ) * kLgQTile + lane * kLgQPitch;
+          const uint4 w0 = *reinterpret_cast<const uint4*>(q), w1 = *reinterpret_cast<const uint4*>(q + 16);
+          ++used;
+          __syncwarp();                      // read by all lanes before the tile is filled again
+          fetch();
+          const uint32_t wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+          const uint32_t sw = word_of(meta, (k >> 1) & 3);
+          // scale (q - 8), at most 8 + 3 significant bits and so exact in fp16:
+          // a nibble in the mantissa of 16.0 is 16 + q, and 24 scale is exact too.
+          // The pairs are (q_i, q_i+4) of a word; x is laid out alike.
+          const __half2 s2 = __float2half2_rn((k & 1 ? bf_hi(sw) : bf_lo(sw)) * wsc),
+                        m24 = __hmul2(s2, __float2half2_rn(-24.0f));
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            const uint32_t v[4] = {wv[w] << 6, wv[w] << 2, wv[w] >> 2, wv[w] >> 6};
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+              av[4 * w + p] = h2u(__hfma2(u2h((v[p] & 0x03C003C0u) | 0x4C004C00u), s2, m24));
+          }
+        } else {
+          // the biases of 64 groups
+          const uint32_t* b =
+              a.wbias + ((size_t)(o >> 7) * (nkv - nk) + (size_t)(k_lo + c - nk)) * 32 * 128 + (row & 127);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) av[e] = __ldcg(b + e * 128);
+        }
+        if (!slot_free(oc)) return false;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) put(st, u, av[4 * u], av[4 * u + 1], av[4 * u + 2], av[4 * u + 3]);
+        slot_done(st);
+        return true;
+      };
+      // ---- a stage of adapters: a block of 64 columns, four pieces of 16 rows ----
+      const int vpl = v_planes(npad), vps = v_passes(npad), passes = BPARTS * vps;
+      auto block_of = [&](int c) { return rank_c + (c - nkm) / passes * split; };
+      const int c_first = nkm + ((nkm ^ grp) & 1);   // this group's first such stage
+      LgAhead& ahead = S.ahead[warp - 2];
+      if (c_first < total) {
+        // its lists, beside the stages of weights
+        const unsigned char* from = nullptr;
+        unsigned char* to = nullptr;
+        if (lane < 2) {
+          from = reinterpret_cast<const unsigned char*>(a.gran + (size_t)(tile / mt) * a.gran_stride + block_of(c_first) * 4) +
+                 lane * 16;
+          to = reinterpret_cast<unsigned char*>(ahead.gran) + lane * 16;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to)), "l"(from) : "memory");
+        }
+        const int n = (row & 96) + (lane >> 4) * 128 + (lane & 15) * 2;   // two tokens a lane
+        if (n < npad) {
+          from = reinterpret_cast<const unsigned char*>(a.tok + tn + n);
+          to = reinterpret_cast<unsigned char*>(&ahead.tok[lane >> 4][(lane & 15) * 2]);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to)), "l"(from) : "memory");
+        }
       }
-      if (!ok) break;
+      auto adapters = [&](int c) -> bool {
+        const uint32_t oc = os + (uint32_t)c;
+        const int st = (int)(oc % kLgRO);
+        const int blk = block_of(c), pass = (c - nkm) % passes, p0 = pass % vps * vpl;
+        const bool lo_part = pass >= vps;
+        const bool here = c == c_first;
+        if (here) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          __syncwarp();
+        }
+        const int2* gran = a.gran + (size_t)(tile / mt) * a.gran_stride + blk * 4;
+        int left[4];                         // rows of the adapter from this piece on, 0: no piece
+        uint4 raw[4][2];
+        int2 tk[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int n = row + 128 * i;
+          tk[i] = n >= npad ? make_int2(0, 0) : here ? ahead.tok[i][lane] : __ldcg(a.tok + tn + n);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int2 gr = blk * 4 + q >= ng ? make_int2(0, 0) : here ? ahead.gran[q] : __ldcg(gran + q);
+          raw[q][0] = raw[q][1] = make_uint4(0, 0, 0, 0);
+          left[q] = live ? gr.y >> 16 : 0;
+          if (left[q] > 0) {
+            const int jq = gr.y & 0xFFFF;
+            const uint16_t* at =
+                static_cast<const uint16_t*>(a.b) + (size_t)gr.x * a.b_stride + (size_t)o * a.rank + jq;
+            if (a.b_vec && jq + 16 <= a.rank) {
+              raw[q][0] = __ldg(reinterpret_cast<const uint4*>(at));
+              raw[q][1] = __ldg(reinterpret_cast<const uint4*>(at) + 1);
+            } else {
+              uint32_t h[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) h[e] = e < left[q] ? at[e] : 0u;
+              raw[q][0] = make_uint4(pack2(h[0], h[1]), pack2(h[2], h[3]), pack2(h[4], h[5]), pack2(h[6], h[7]));
+              raw[q][1] = make_uint4(pack2(h[8], h[9]), pack2(h[10], h[11]), pack2(h[12], h[13]), pack2(h[14], h[15]));
+            }
+          }
+        }
+        if (!slot_free(oc)) return false;
+        // ---- v: each token's planes in its own columns, zeros elsewhere ----
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int n = row + 128 * i;
+          if (n >= npad) continue;
+          const int q0 = tk[i].x - blk * 4, q1 = q0 + tk[i].y;   // its pieces in the block's numbers
+          const uint16_t* v = reinterpret_cast<const uint16_t*>(a.v) +
+                              ((size_t)(tn + n) * C::NV + p0) * a.v_stride - q0 * 16;
+          unsigned char* at = stages + (size_t)st * kLgStage + kLgA + (size_t)n * 128;
+          for (int p = 0; p < vpl && p0 + p < C::NV; ++p) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const bool in = (u >> 1) >= q0 && (u >> 1) < q1;
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                               smem_addr(at + (size_t)p * npad * 128 + ((u ^ (n & 7)) << 4))),
+                           "l"(in ? v + (size_t)p * a.v_stride + u * 8 : reinterpret_cast<const uint16_t*>(a.v)),
+                           "r"(in ? 16 : 0)
+                           : "memory");
+            }
+          }
+        }
+        // ---- B ----
+        const uint32_t wsc2 = pack_bf2(wsc, wsc);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t w[8] = {raw[q][0].x, raw[q][0].y, raw[q][0].z, raw[q][0].w,
+                           raw[q][1].x, raw[q][1].y, raw[q][1].z, raw[q][1].w};
+          if (left[q] < 16) {
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+              w[p] &= (2 * p < left[q] ? 0xFFFFu : 0u) | (2 * p + 1 < left[q] ? 0xFFFF0000u : 0u);
+          }
+          // a non-finite value must not meet the zeros of other tokens: an
+          // exponent of all ones carries into the sign place
+          constexpr uint32_t kExp = AT == 2 ? 0x7C007C00u : 0x7F807F80u, kOne = AT == 2 ? 0x04000400u : 0x00800080u;
+          uint32_t any = 0;
+#pragma unroll
+          for (int p = 0; p < 8; ++p) any |= (w[p] & kExp) + kOne;
+          if (any & 0x80008000u) {
+            S.bad = 1;
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+              const uint32_t b = ((w[p] & kExp) + kOne) & 0x80008000u;
+              w[p] &= ~((b >> 15) * 0xFFFFu);
+            }
+          }
+#pragma unroll
+          for (int p = 0; p < 8; ++p) {
+            if constexpr (AT == 2) {
+              float w0, w1;
+              unpack2<AT>(w[p], w0, w1);
+              w0 *= wsc;
+              w1 *= wsc;
+              w[p] = pack_bf2(w0, w1);
+              if (lo_part) w[p] = pack_bf2(w0 - bf_lo(w[p]), w1 - bf_hi(w[p]));
+            } else {
+              w[p] = bf2_fma(w[p], wsc2, 0x80008000u);   // a power of two: exact
+            }
+          }
+          put(st, 2 * q, w[0], w[1], w[2], w[3]);
+          put(st, 2 * q + 1, w[4], w[5], w[6], w[7]);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        slot_done(st);
+        return true;
+      };
+      for (int c = grp; c < total && ok; c += 2) ok = c < nkm ? weights(c) : adapters(c);
       os += (uint32_t)total;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     // ---------------- epilogue ----------------
-    const int quad = warp & 3, half = (warp - 2 - kLgConv) >> 2;
+    const int quad = warp & 3;               // the quarter of tensor memory a warp can reach
+    const int half = (warp - 2 - kLgConv) >> 2;   // 16-token pieces half, half + 2, ...
     const int row = quad * 32 + lane;
-    const int n_mine = (warp - 2 - kLgConv) * 32 + lane;  // the token this thread lists
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-    uint32_t eb = 0, gq = 0;
-    // all epilogue warps meet (bounded, unlike a named barrier)
-    auto meet = [&]() -> bool {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&S.epi);
-      const bool w = warp_wait(&S.epi, eb & 1, abort, a.status);
-      ++eb;
-      return w;
-    };
-    int ti = 0;
-    for (int tile = first_tile; tile < tiles; tile += step, ++ti) {
-      LgList& L = S.list[ti & 1];
-      const long long tb = (long long)(tile / mt) * a.NT;
-      const int ntok = tokens_of(tile), npad = (ntok + 15) & ~15;
-      const int o = (tile % mt) * kLgM + row;
-      // ---- the tile's adapters: first token of each, pieces of 16 rows ----
-      int rank = 0, id = -1;
-      if (a.adapter && n_mine < ntok) id = adapter_of(a, tb + n_mine, rank);
-      L.id[n_mine] = id;
-      L.rank[n_mine] = (uint16_t)rank;
-      if (!meet()) break;
-      int first = n_mine;
-      if (id >= 0 && rank > 0) {
-        const int4* ids4 = reinterpret_cast<const int4*>(L.id);
-        for (int j = 0; j * 4 < n_mine; ++j) {
-          const int4 v = ids4[j];
-          const int f = v.x == id ? 0 : v.y == id ? 1 : v.z == id ? 2 : v.w == id ? 3 : 4;
-          if (f < 4) {
-            first = min(first, j * 4 + f);
-            break;
-          }
-        }
-      }
-      L.first[n_mine] = id >= 0 && rank > 0 ? (uint16_t)first : (uint16_t)0xFFFF;
-      const int mine = id >= 0 && rank > 0 && first == n_mine ? (rank + 15) >> 4 : 0;
-      int incl = mine;
-#pragma unroll
-      for (int s = 1; s < 32; s <<= 1) {
-        const int up = __shfl_up_sync(kAllLanes, incl, s);
-        if (lane >= s) incl += up;
-      }
-      if (lane == 31) L.wsum[warp - 2 - kLgConv] = incl;
-      if (!meet()) break;
-      int base = 0, all = 0;
-      for (int w = 0; w < kLgEpi; ++w) {
-        if (w < warp - 2 - kLgConv) base += L.wsum[w];
-        all += L.wsum[w];
-      }
-      L.goff[n_mine] = (uint16_t)(base + incl - mine);
-      for (int i = 0; i < mine; ++i) L.gran[base + incl - mine + i] = (uint16_t)(n_mine << 4 | i);
-      if (n_mine == 0) L.n_gran = all;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&S.listfull[ti & 1]);
-      if (ti == 0) pdl_wait();  // what the prep kernel wrote; y may still be read before it
-      const int ew = a.ew[o];
-      if (half == 0) S.ew[row] = ew;
-      L.fx[n_mine] = n_mine < ntok ? pow2(a.ex[tb + n_mine]) : 0.0f;
-      if (!meet()) break;
-      const int total = nkm + lora_stages(all, npad);
+    uint32_t gq = 0;
+    pdl_wait();
+    for (int tile = first_tile; tile < tiles; tile += step) {
+      const int o = (tile % mt) * M + row;
       const bool live = o < a.N;
-      float* part = reinterpret_cast<float*>(stages);  // split: [token][128 rows]
-      // a sum times 2^(ew + ex): within range in this order, as |ew| above 60
-      // is taken in two steps
+      const long long tn = (long long)(tile / mt) * a.NT;
+      const int ntok = tokens_of(tile), npad = (ntok + 15) & ~15;
+      const int ew = __ldcg(a.ew + o);
+      const int total = stages_of(npad, pieces_at(tile));
+      // the exponents of this warp's tokens, 16 of each piece in the first and
+      // in the last lanes, before there is a sum to wait for
+      int exr[C::NMAX / 32];
+#pragma unroll
+      for (int i = 0; i < C::NMAX / 32; ++i) {
+        const int n0 = (half + 2 * i) * 16;
+        exr[i] = n0 < npad ? __ldcg(a.ex + tn + n0 + (lane & 15)) : 0;
+      }
+      auto sum_wait = [&]() {
+        if (!lg_warp_wait(&S.accfull[gq & 1], (gq >> 1) & 1, abort, a.status)) return false;
+        fence_after();
+        return true;
+      };
+      auto sum_done = [&]() {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.accempty[gq & 1]);
+        ++gq;
+      };
+      // a sum times 2^(ew + ex): within range in this order, as |ew| above 60 is
+      // taken in two steps
       const int ewc = max(-60, min(60, ew));
       const float fw = pow2(ewc), fr = pow2(ew - ewc);
-      // 16 columns of sums to y
-      auto put16 = [&](int n0, const float (&v)[16]) {
-        if (!live) return;
-        float fx[16];
+      float* part = reinterpret_cast<float*>(stages);   // split: [token][M rows]
+      auto put16 = [&](int n0, int ex, const float (&v)[16]) {
+        if (split > 1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float4 f = *reinterpret_cast<const float4*>(&L.fx[n0 + 4 * e]);
-          fx[4 * e] = f.x;
-          fx[4 * e + 1] = f.y;
-          fx[4 * e + 2] = f.z;
-          fx[4 * e + 3] = f.w;
+          for (int e = 0; e < 16; ++e) part[(n0 + e) * M + row] = v[e];
+          return;
         }
-        const size_t at = (size_t)(tb + n0) * a.y_stride + o;
+        const float fx = pow2(ex);
+        const size_t at = (size_t)(tn + n0) * a.y_stride + o;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          float r = v[e] * fw * fx[e];
+          float r = v[e] * fw * __shfl_sync(kAllLanes, fx, e);
           if (ew != ewc) r *= fr;
-          if (n0 + e < ntok) store_val<XT>(a.y, at + (size_t)e * a.y_stride, r);
+          if (live && n0 + e < ntok) store_val<XT>(a.y, at + (size_t)e * a.y_stride, r);
         }
       };
       if constexpr (F32) {
-        float acc[4][16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
+        float acc[4][16] = {};
         bool ok = true;
-        for (int c = 0; c < total; c += C::GROUP, ++gq) {
-          const int b = (int)(gq & 1);
-          if (!warp_wait(&S.accfull[b], (gq >> 1) & 1, abort, a.status)) {
-            ok = false;
-            break;
-          }
-          fence_after();
+        for (int c = 0; c < total && ok; c += C::GROUP) {
+          ok = sum_wait();
+          if (!ok) break;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int n0 = (2 * i + half) * 16;
+            const int n0 = (half + 2 * i) * 16;
             if (n0 < npad) {
               uint32_t d[16];
-              ld16(tmem + lane_addr + (uint32_t)(b * 128 + n0), d);
+              ld16(tmem + lane_addr + (gq & 1) * 256 + (uint32_t)n0, d);
               wait_ld();
 #pragma unroll
               for (int e = 0; e < 16; ++e) acc[i][e] += __uint_as_float(d[e]);
             }
           }
-          fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&S.accempty[b]);
+          sum_done();
         }
         if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n0 = (2 * i + half) * 16;
-          if (n0 >= npad) continue;
-          if (split > 1) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) part[(n0 + e) * kLgM + row] = acc[i][e];
-          } else {
-            put16(n0, acc[i]);
-          }
-        }
+        for (int i = 0; i < 4; ++i)
+          if ((half + 2 * i) * 16 < npad) put16((half + 2 * i) * 16, exr[i], acc[i]);
       } else {
-        const int b = nbuf == 2 ? (int)(gq & 1) : 0;
-        if (!warp_wait(&S.accfull[b], (nbuf == 2 ? gq >> 1 : gq) & 1, abort, a.status)) break;
-        fence_after();
-        ++gq;
-        for (int n0 = half * 16; n0 < npad; n0 += 32) {
+        if (!sum_wait()) break;
+#pragma unroll
+        for (int i = 0; i < C::NMAX / 32; ++i) {
+          const int n0 = (half + 2 * i) * 16;
+          if (n0 >= npad) continue;
           uint32_t d[16];
-          ld16(tmem + lane_addr + (uint32_t)(b * 128 + n0), d);
+          ld16(tmem + lane_addr + (gq & 1) * 256 + (uint32_t)n0, d);
           wait_ld();
           float v[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(d[e]);
-          if (split > 1) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) part[(n0 + e) * kLgM + row] = v[e];
-          } else {
-            put16(n0, v);
-          }
+          put16(n0, exr[i], v);
         }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.accempty[b]);
+        sum_done();
       }
-      // terms that are not finite, after the fact: they decide their values
-      if (S.bad && split == 1 && live)
-        for (int n = half * 16; n < ntok; n += (n & 15) == 15 ? 17 : 1)
-          if (L.first[n] != 0xFFFF) add_bad_terms<XT, AT>(a, L.id[n], L.rank[n], o, tb + n);
+      if (split > 1) {
+        if (half == 0) S.ew[row] = ew;
+      } else if (live && S.bad && a.adapter) {
+        // terms that are not finite, after the fact: they decide their values
+        for (int n0 = half * 16; n0 < ntok; n0 += 32)
+          for (int n = n0; n < min(n0 + 16, ntok); ++n) add_bad_terms<XT, AT>(a, o, tn + n);
+      }
     }
   }
   if (split > 1) {
     // the cluster's partial sums, each CTA a share of the tokens, added in the order of K
     __syncwarp();
     cluster_sync_all();
-    const LgList& L = S.list[0];
     const int tile = first_tile, ntok = tokens_of(tile);
-    const long long tb = (long long)(tile / mt) * a.NT;
+    const long long tn = (long long)(tile / mt) * a.NT;
     const int n_lo = ntok * rank_c / split, n_hi = ntok * (rank_c + 1) / split;
     bool bad = false;
     for (int r = 0; r < split; ++r) bad |= ld_cluster_i(map_rank(smem_addr(&S.bad), (uint32_t)r)) != 0;
-    for (int i = tid; i < (n_hi - n_lo) * kLgM; i += kLgThreads) {
-      const int n = n_lo + i / kLgM, row = i % kLgM, o = (tile % mt) * kLgM + row;
+    for (int i = tid; i < (n_hi - n_lo) * M; i += kLgThreads) {
+      const int n = n_lo + i / M, row = i % M, o = (tile % mt) * M + row;
       if (o >= a.N || S.abort) continue;
-      const uint32_t at = smem_addr(stages) + (uint32_t)(n * kLgM + row) * 4;
+      const uint32_t at = smem_addr(stages) + (uint32_t)(n * M + row) * 4;
       float p[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) p[r] = r < split ? ld_cluster(map_rank(at, (uint32_t)r)) : 0.0f;
@@ -1312,9 +1538,9 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
 #pragma unroll
       for (int r = 1; r < 8; ++r) v += p[r];
       const int ew = S.ew[row], ewc = max(-60, min(60, ew));
-      v = v * pow2(ewc) * L.fx[n] * pow2(ew - ewc);
-      store_val<XT>(a.y, (size_t)(tb + n) * a.y_stride + o, v);
-      if (bad && L.first[n] != 0xFFFF) add_bad_terms<XT, AT>(a, L.id[n], L.rank[n], o, tb + n);
+      v = v * pow2(ewc) * pow2(__ldcg(a.ex + tn + n)) * pow2(ew - ewc);
+      store_val<XT>(a.y, (size_t)(tn + n) * a.y_stride + o, v);
+      if (bad && a.adapter) add_bad_terms<XT, AT>(a, o, tn + n);
     }
     cluster_sync_all();  // no CTA ends while another reads its sums
   }
@@ -1331,17 +1557,17 @@ bool decodes(const LoraArgs& a) {
 
 // Tokens per tile and CTAs per tile (K and the adapters split over a cluster):
 // the smallest of a plain estimate in clocks.  A stage costs its matrix steps
-// (N / 2 clocks each, 4 per plane of x) or the conversion of its 128 x 64
-// weights, whichever is longer; a stage of adapters, of which a tile of few
-// tokens may have one for every few tokens, about twice that; a tile adds its
-// epilogue, a split the exchange of the sums.
+// (N / 2 clocks each, 4 per plane of x), what it moves through shared memory at
+// 128 bytes a clock, or the conversion of its weights, whichever is longest; a
+// stage of adapters, of which a tile of few tokens may have one for every few
+// tokens, about 1500; a tile adds its epilogue, a split the exchange of the sums.
 void lg_shape(const LoraArgs& a, int sms, int* NT, int* split) {
   const bool f32 = a.x_type == 0;
-  const int nmax = f32 ? 128 : 256, nk = a.K >> 6;
-  const long long mt = (a.N + kLgM - 1) / kLgM;
+  const int nmax = f32 ? 128 : 256, nk = a.K >> 6, pl = f32 ? 2 : 1;
   double best = 1e300;
   *NT = 16;
   *split = 1;
+  const long long mt = (a.N + kLgM - 1) / kLgM;
   for (int n = 16; n <= nmax; n += 16) {
     if (n > 16 && n - 16 >= a.tokens) break;
     const long long tiles = mt * ((a.tokens + n - 1) / n);
@@ -1349,13 +1575,14 @@ void lg_shape(const LoraArgs& a, int sms, int* NT, int* split) {
     if (a.adapter) {
       const int nv = f32 ? 3 : 2, per = 256 / n < nv ? 256 / n : nv, passes = (nv + per - 1) / per;
       const double many = a.tokens <= 512 ? (a.count < n ? a.count : n) : 2.0;
-      lora = passes * (many * ((a.rank + 15) / 16) / 4.0 + 0.5);
+      lora = (a.a_type == 2 ? 2 : 1) * passes * (many * ((a.rank + 15) / 16) / 4.0 + 0.5);
     }
     for (int s = 1; s <= 8; s *= 2) {
       if (s > nk || (s > 1 && tiles * s > (s == 8 ? 128 : sms))) break;
       const double waves = (double)((tiles * s + sms - 1) / sms);
-      const double mma = (f32 ? 4.0 : 2.0) * n, stage = mma > 450.0 ? mma : 450.0;
-      const double t = waves * (((nk + s - 1) / s) * stage + (lora / s) * (2.0 * stage + 300.0) + 1500.0 + 10.0 * n +
+      const double smem = (4.0 * pl * (4096.0 + 32.0 * n) + 20480.0 + 128.0 * n * pl) / 128.0;
+      const double stage = smem > 400.0 ? smem : 400.0;
+      const double t = waves * (((nk + s - 1) / s) * stage + (lora / s) * 1500.0 + 2000.0 + 10.0 * n +
                                 (s > 1 ? 1500.0 : 0.0));
       if (t < best) {
         best = t;
@@ -1406,9 +1633,16 @@ cudaError_t launch(const LoraArgs& a, int sms, cudaStream_t s, uint64_t* launche
   const bool dec = decodes(a);
   const long long rows = (a.tokens + 15) / 16 * 16;
   const long long row_blocks = dec ? 0 : a.row_threads == 32 ? rows / kPrepWarps : rows;
-  const long long prep = a.v_blocks + a.w_blocks + row_blocks;
+  const long long prep = a.v_blocks + a.l_blocks + a.w_blocks + row_blocks;
+  if (a.after_v) {
+    const cudaError_t e = launch_cfg(lora_v_kernel<XT, AT>, (unsigned)a.after_v, VBig<XT>::THREADS, VBig<XT>::BYTES, 1,
+                                     s, a);
+    if (e != cudaSuccess) return e;
+    if (launches) *launches += 1;
+  }
   if (prep) {
-    const cudaError_t e = launch_cfg(lora_prep_kernel<XT, AT>, (unsigned)prep, kPrepThreads, 0, 1, s, a);
+    const cudaError_t e = launch_cfg(lora_prep_kernel<XT, AT>, (unsigned)prep, kPrepThreads, a.v_blocks ? kPrepRed : 0, 1,
+                                     s, a);
     if (e != cudaSuccess) return e;
     if (launches) *launches += 1;
   }
@@ -1454,19 +1688,32 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
     a.wbias = reinterpret_cast<uint32_t*>(base + off);
     off += up((size_t)a.w_blocks * (a.x_type == 0 ? 2 : 1) * ((nk + 63) / 64) * 32 * kLgM * 4);
   }
-  a.v_blocks = 0;
+  a.v_blocks = a.l_blocks = a.after_v = 0;
   a.v_stride = 0;
   a.v_slots = 1;
   if (a.adapter) {
     a.v_stride = ((size_t)a.rank + 15) / 16 * 16;
-    // tiles of 16 tokens while a tile's adapters are worth blocks of their own,
-    // of 32 where a prompt's tokens share them
-    a.v_tile = a.tokens >= 1024 ? 32 : 16;
     a.v_planes = dec ? 0 : a.x_type == 0 ? 3 : 2;
-    const long long vt = (a.tokens + a.v_tile - 1) / a.v_tile;
     const long long most = a.tokens < a.count ? a.tokens : a.count;
-    if (a.v_tile == 16) a.v_slots = (int)(most < 16 ? most : 16);
-    a.v_blocks = (int)(vt * a.v_slots);
+    // v: tiles of 16 tokens in the prep kernel while a tile's adapters are worth
+    // blocks of their own, a kernel of its own where a prompt's tokens share them
+    if (a.tokens < 1024) {
+      a.v_slots = (int)(most < 16 ? most : 16);
+      a.v_blocks = (int)((a.tokens + 15) / 16 * a.v_slots);
+    } else {
+      a.v_slots = (int)(most < 4 ? most : 4);
+      a.after_v = (int)((a.tokens + 31) / 32 * a.v_slots);
+    }
+    if (!dec) {
+      a.l_blocks = (int)((a.tokens + a.NT - 1) / a.NT);
+      a.gran_stride = (size_t)a.NT * ((a.rank + 15) / 16);
+      a.gran = reinterpret_cast<int2*>(base + off);
+      off += up((size_t)a.l_blocks * a.gran_stride * 8);
+      a.tok = reinterpret_cast<int2*>(base + off);
+      off += up((size_t)((a.tokens + 15) / 16 * 16) * 8);
+      a.n_gran = reinterpret_cast<int*>(base + off);
+      off += up((size_t)a.l_blocks * 4);
+    }
     a.v = reinterpret_cast<float*>(base + off);
     off += up((size_t)a.tokens * a.v_stride * (dec ? 4 : 2 * a.v_planes));
   }
@@ -1475,7 +1722,8 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
 
 template <int XT, int AT>
 cudaError_t set_smem() {
-  cudaError_t e = cudaFuncSetAttribute(lora_gemm_kernel<XT, AT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLgSmem);
+  cudaError_t e = cudaFuncSetAttribute(lora_v_kernel<XT, AT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)VBig<XT>::BYTES);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(lora_gemm_kernel<XT, AT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLgSmem);
   auto dec = [&](auto kernel) {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kDecSmem);
   };
