@@ -36,6 +36,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "osm_common.cuh"
 #include "osm_kernels.cuh"
 #include "osm_tcgen05.cuh"
@@ -341,15 +343,40 @@ __device__ __forceinline__ void prep_v(const LoraArgs& a, int block, float* red,
   }
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ int ld_cluster_i(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 // Many tokens: tiles of 32, so that a prompt's tokens share the rows of A; K in
 // stages of 64 through shared memory (rows of x and A as they are, padded so
 // that a warp's 16-byte reads meet all banks), 2 x 2 warps of 16 tokens by 32
 // rows of A.  Rows of other adapters are not loaded: they mean nothing in x's
-// part and their sums are not stored.  Bound by the matrix steps (8 clocks each
-// per quarter of an SM) for fp32 rows, by the reads of x for the others.
+// part and their sums are not stored; neither do rows behind the rank.  A
+// cluster of 4 CTAs splits K and adds its sums, in the order of K: with one CTA
+// per tile an SM has 4 warps to hide every latency.
 template <int XT>
 struct VBig {
-  static constexpr int TOK = 32, COLS = 64, STAGES = 4, THREADS = 128;
+  static constexpr int TOK = 32, COLS = 64, STAGES = 3, THREADS = 128, KSPLIT = 4;
   static constexpr int XPITCH = XT == 0 ? 272 : 192, APITCH = 192;   // bytes
   static constexpr size_t STAGE = (size_t)TOK * XPITCH + (size_t)COLS * APITCH;
   static constexpr size_t BYTES = STAGES * STAGE;
@@ -359,16 +386,17 @@ __global__ void __launch_bounds__(VBig<XT>::THREADS) lora_v_kernel(const __grid_
   extern __shared__ uint4 v_smem[];
   __shared__ VShared S;
   unsigned char* const sm = reinterpret_cast<unsigned char*>(v_smem);
-  const int block = (int)blockIdx.x;
+  using B = VBig<XT>;
+  const int block = (int)blockIdx.x / B::KSPLIT, krank = (int)cluster_rank();
   pdl_wait();
   pdl_trigger();
-  using B = VBig<XT>;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int v_tiles = (int)((a.tokens + B::TOK - 1) / B::TOK), slot = block / v_tiles;   // as in prep_v
   const long long t0 = (long long)(block % v_tiles) * B::TOK;
   list_adapters<B::TOK>(a, t0, S);
   const int g = lane >> 2, q = lane & 3, wm = warp & 1, wn = warp >> 1;
-  const int r0 = wm * 16 + g, steps = a.K / 64;
+  const int r0 = wm * 16 + g;
+  const int s_lo = a.K / 64 * krank / B::KSPLIT, steps = a.K / 64 * (krank + 1) / B::KSPLIT - s_lo;
   constexpr int XB = XT == 0 ? 4 : 2, XU = XT == 0 ? 16 : 8;   // bytes of a value, 16-byte pieces of a row's stage
   constexpr int NX = B::TOK * XU / B::THREADS, NA = B::COLS * 8 / B::THREADS;   // pieces per thread and stage
   auto copy16 = [&](unsigned char* to, const unsigned char* from, bool vec, int align) {
@@ -396,13 +424,13 @@ __global__ void __launch_bounds__(VBig<XT>::THREADS) lora_v_kernel(const __grid_
       for (int e = 0; e < NX; ++e) {
         const int i = tid + e * B::THREADS, r = i / XU, u = i % XU;
         px[e] = S.id[r] == id
-                    ? static_cast<const unsigned char*>(a.x) + (size_t)(t0 + r) * a.x_stride * XB + u * 16 : nullptr;
+                    ? static_cast<const unsigned char*>(a.x) + ((size_t)(t0 + r) * a.x_stride + s_lo * 64) * XB + u * 16 : nullptr;
       }
 #pragma unroll
       for (int e = 0; e < NA; ++e) {
         const int i = tid + e * B::THREADS, r = i >> 3, u = i & 7;
         pa[e] = j0 + r < rank ? static_cast<const unsigned char*>(a.a) +
-                                    ((size_t)id * a.a_stride + (size_t)(j0 + r) * a.K) * 2 + u * 16 : nullptr;
+                                    ((size_t)id * a.a_stride + (size_t)(j0 + r) * a.K + s_lo * 64) * 2 + u * 16 : nullptr;
       }
       auto load = [&](int st) {
         if (st < steps) {
@@ -457,7 +485,6 @@ __global__ void __launch_bounds__(VBig<XT>::THREADS) lora_v_kernel(const __grid_
             for (int s = 0; s < 2; ++s)
 #pragma unroll
               for (int n = 0; n < 4; ++n)
-                if (j0 + wn * 32 + n * 8 < rank)
                   mma16<XT>(acc[n], xa.w[2 * s], xb.w[2 * s], xa.w[2 * s + 1], xb.w[2 * s + 1], w[n].w[2 * s],
                             w[n].w[2 * s + 1]);
           } else {
@@ -479,7 +506,6 @@ __global__ void __launch_bounds__(VBig<XT>::THREADS) lora_v_kernel(const __grid_
               }
 #pragma unroll
               for (int n = 0; n < 4; ++n) {
-                if (j0 + wn * 32 + n * 8 >= rank) continue;
                 float b0, b1;
                 raw_pair<AT>(w[n], s, b0, b1);
                 if constexpr (XT == 0)
@@ -498,22 +524,41 @@ __global__ void __launch_bounds__(VBig<XT>::THREADS) lora_v_kernel(const __grid_
         m1 = fmaxf(lo, hi);
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
-      __syncthreads();   // all stages read before the next adapter's loads
-      if (!work) continue;
+      __syncthreads();   // all stages read: their memory takes the sums
+      float* red = reinterpret_cast<float*>(sm);   // [token][COLS], then each token's largest |x|
       m0 = fmaxf(m0, __shfl_xor_sync(kAllLanes, m0, 1));
       m0 = fmaxf(m0, __shfl_xor_sync(kAllLanes, m0, 2));
       m1 = fmaxf(m1, __shfl_xor_sync(kAllLanes, m1, 1));
       m1 = fmaxf(m1, __shfl_xor_sync(kAllLanes, m1, 2));
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const int j = j0 + wn * 32 + n * 8 + 2 * q;
-        if (j >= ((rank + 15) & ~15)) continue;   // whole pieces of 16: zeros behind the adapter's rank
-        const bool c0 = j < rank, c1 = j + 1 < rank;
-        if (in0)
-          store_planes(a, t0 + r0, j, c0 ? gain * acc[n][0] : 0.0f, c1 ? gain * acc[n][1] : 0.0f, row_exponent(m0));
-        if (in1)
-          store_planes(a, t0 + r0 + 8, j, c0 ? gain * acc[n][2] : 0.0f, c1 ? gain * acc[n][3] : 0.0f, row_exponent(m1));
+        float* at = red + (size_t)r0 * B::COLS + wn * 32 + n * 8 + 2 * q;
+        *reinterpret_cast<float2*>(at) = make_float2(acc[n][0], acc[n][1]);
+        *reinterpret_cast<float2*>(at + 8 * B::COLS) = make_float2(acc[n][2], acc[n][3]);
       }
+      if (wn == 0 && q == 0) {
+        red[B::TOK * B::COLS + r0] = m0;
+        red[B::TOK * B::COLS + r0 + 8] = m1;
+      }
+      __syncwarp();
+      cluster_sync_all();
+      // this CTA's quarter of the tokens, pairs of columns
+      constexpr int MINE = B::TOK / B::KSPLIT;
+      for (int o = tid; o < MINE * B::COLS / 2; o += B::THREADS) {
+        const int r = krank * MINE + o / (B::COLS / 2), c = o % (B::COLS / 2) * 2, j = j0 + c;
+        if (S.id[r] != id || j >= ((rank + 15) & ~15)) continue;   // whole pieces of 16: zeros behind the rank
+        float v0 = 0.0f, v1 = 0.0f, m = 0.0f;
+#pragma unroll
+        for (int z = 0; z < B::KSPLIT; ++z) {
+          const uint32_t at = map_rank(smem_addr(red), (uint32_t)z);
+          v0 += ld_cluster(at + (uint32_t)(r * B::COLS + c) * 4);
+          v1 += ld_cluster(at + (uint32_t)(r * B::COLS + c) * 4 + 4);
+          m = fmaxf(m, ld_cluster(at + (uint32_t)(B::TOK * B::COLS + r) * 4));
+        }
+        store_planes(a, t0 + r, j, j < rank ? gain * v0 : 0.0f, j + 1 < rank ? gain * v1 : 0.0f, row_exponent(m));
+      }
+      __syncwarp();
+      cluster_sync_all();   // read by all before the next sums
     }
   }
 }
@@ -916,6 +961,7 @@ struct alignas(16) LgAhead {
 };
 struct LgShared {
   LgAhead ahead[kLgConv];
+  float fx[kLgEpi][128];    // 2^exponent of an epilogue warp's tokens
   int ew[kLgM];             // exponents of the tile's rows of W
   int bad;                  // some B held a non-finite value
   volatile int abort;
@@ -924,29 +970,6 @@ struct LgShared {
 };
 constexpr size_t kLgSmem = kLgRO * kLgStage + kLgConv * kLgRQ * kLgQTile + sizeof(LgShared) + 1024;
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ int ld_cluster_i(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
@@ -988,13 +1011,18 @@ __device__ __noinline__ void add_bad_terms(const LoraArgs& a, int o, long long t
 // status bit is set and the CTA-wide abort flag makes all later waits return.
 // It counts clocks, not the global timer, whose read takes long enough to show
 // on every wait that does not succeed at once.
+// NAP: the waiting warp stays off the issue slots between polls (waits that are
+// long and not on the way of the matrix steps).
+template <bool NAP = false>
 __device__ __forceinline__ bool lg_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t* status) {
   if (mbar_try_sleep(bar, parity)) return true;
   const long long t0 = clock64();
   for (;;) {
 #pragma unroll 1
-    for (int i = 0; i < 64; ++i)
+    for (int i = 0; i < 64; ++i) {
+      if (NAP) __nanosleep(200);
       if (mbar_try_sleep(bar, parity)) return true;
+    }
     if (*abort) return false;
     if (clock64() - t0 > 4000000000ll) break;
   }
@@ -1003,8 +1031,9 @@ __device__ __forceinline__ bool lg_wait(uint64_t* bar, uint32_t parity, volatile
   return false;
 }
 // By a whole warp, with one outcome for all its lanes.
+template <bool NAP = false>
 __device__ __forceinline__ bool lg_warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t* status) {
-  return __all_sync(kAllLanes, lg_wait(bar, parity, abort, status));
+  return __all_sync(kAllLanes, lg_wait<NAP>(bar, parity, abort, status));
 }
 
 // D[tmem] (+)= A[smem desc] * B[smem desc]
@@ -1431,16 +1460,18 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
       const int ntok = tokens_of(tile), npad = (ntok + 15) & ~15;
       const int ew = __ldcg(a.ew + o);
       const int total = stages_of(npad, pieces_at(tile));
-      // the exponents of this warp's tokens, 16 of each piece in the first and
-      // in the last lanes, before there is a sum to wait for
-      int exr[C::NMAX / 32];
+      // 2^exponent of this warp's tokens, piece by piece, before there is a sum
+      // to wait for
+      float* fx = S.fx[warp - 2 - kLgConv];
+      __syncwarp();
 #pragma unroll
-      for (int i = 0; i < C::NMAX / 32; ++i) {
-        const int n0 = (half + 2 * i) * 16;
-        exr[i] = n0 < npad ? __ldcg(a.ex + tn + n0 + (lane & 15)) : 0;
+      for (int i = 0; i < C::NMAX / 64; ++i) {
+        const int n = (half + 4 * i + (lane >> 4) * 2) * 16 + (lane & 15);
+        fx[32 * i + lane] = n < npad ? pow2(__ldcg(a.ex + tn + n)) : 0.0f;
       }
+      __syncwarp();
       auto sum_wait = [&]() {
-        if (!lg_warp_wait(&S.accfull[gq & 1], (gq >> 1) & 1, abort, a.status)) return false;
+        if (!lg_warp_wait<true>(&S.accfull[gq & 1], (gq >> 1) & 1, abort, a.status)) return false;
         fence_after();
         return true;
       };
@@ -1455,19 +1486,36 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
       const int ewc = max(-60, min(60, ew));
       const float fw = pow2(ewc), fr = pow2(ew - ewc);
       float* part = reinterpret_cast<float*>(stages);   // split: [token][M rows]
-      auto put16 = [&](int n0, int ex, const float (&v)[16]) {
+      using Y = std::conditional_t<F32, float, uint16_t>;
+      auto put16 = [&](int i, const float (&v)[16]) {
+        const int n0 = (half + 2 * i) * 16;
         if (split > 1) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) part[(n0 + e) * M + row] = v[e];
           return;
         }
-        const float fx = pow2(ex);
-        const size_t at = (size_t)(tn + n0) * a.y_stride + o;
+        if (!live) return;
+        float r[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float r = v[e] * fw * __shfl_sync(kAllLanes, fx, e);
-          if (ew != ewc) r *= fr;
-          if (live && n0 + e < ntok) store_val<XT>(a.y, at + (size_t)e * a.y_stride, r);
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const float4 f = *reinterpret_cast<const float4*>(fx + 16 * i + 4 * e4);
+          r[4 * e4] = v[4 * e4] * fw * f.x;
+          r[4 * e4 + 1] = v[4 * e4 + 1] * fw * f.y;
+          r[4 * e4 + 2] = v[4 * e4 + 2] * fw * f.z;
+          r[4 * e4 + 3] = v[4 * e4 + 3] * fw * f.w;
+        }
+        if (ew != ewc) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) r[e] *= fr;
+        }
+        Y* at = static_cast<Y*>(a.y) + (size_t)(tn + n0) * a.y_stride + o;
+        if (n0 + 16 <= ntok) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e, at += a.y_stride) store_val<XT>(at, 0, r[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e, at += a.y_stride)
+            if (n0 + e < ntok) store_val<XT>(at, 0, r[e]);
         }
       };
       if constexpr (F32) {
@@ -1492,7 +1540,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
         if (!ok) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if ((half + 2 * i) * 16 < npad) put16((half + 2 * i) * 16, exr[i], acc[i]);
+          if ((half + 2 * i) * 16 < npad) put16(i, acc[i]);
       } else {
         if (!sum_wait()) break;
 #pragma unroll
@@ -1505,7 +1553,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
           float v[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(d[e]);
-          put16(n0, exr[i], v);
+          put16(i, v);
         }
         sum_done();
       }
@@ -1635,8 +1683,8 @@ cudaError_t launch(const LoraArgs& a, int sms, cudaStream_t s, uint64_t* launche
   const long long row_blocks = dec ? 0 : a.row_threads == 32 ? rows / kPrepWarps : rows;
   const long long prep = a.v_blocks + a.l_blocks + a.w_blocks + row_blocks;
   if (a.after_v) {
-    const cudaError_t e = launch_cfg(lora_v_kernel<XT, AT>, (unsigned)a.after_v, VBig<XT>::THREADS, VBig<XT>::BYTES, 1,
-                                     s, a);
+    const cudaError_t e = launch_cfg(lora_v_kernel<XT, AT>, (unsigned)a.after_v * VBig<XT>::KSPLIT, VBig<XT>::THREADS,
+                                     VBig<XT>::BYTES, VBig<XT>::KSPLIT, s, a);
     if (e != cudaSuccess) return e;
     if (launches) *launches += 1;
   }
@@ -1701,8 +1749,11 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
       a.v_slots = (int)(most < 16 ? most : 16);
       a.v_blocks = (int)((a.tokens + 15) / 16 * a.v_slots);
     } else {
-      a.v_slots = (int)(most < 4 ? most : 4);
-      a.after_v = (int)((a.tokens + 31) / 32 * a.v_slots);
+      // one cluster per tile for all of its adapters where the tiles fill the
+      // GPU (clusters without an adapter cost about as much as their launch)
+      const long long vt = (a.tokens + 31) / 32, fill = sms / vt;
+      a.v_slots = (int)(fill < 1 ? 1 : fill < most ? fill : most);
+      a.after_v = (int)(vt * a.v_slots);
     }
     if (!dec) {
       a.l_blocks = (int)((a.tokens + a.NT - 1) / a.NT);
