@@ -448,6 +448,9 @@ struct RouteArgs {
   float* weights;           // [tokens][k]
   float* mass;              // [tokens] or null
   uint32_t* status;
+  // filled by launch_route_scores: lanes per group, experts per lane, whether
+  // a lane's run is read in 16-byte vectors
+  int lanes, chunk, vec;
 };
 cudaError_t launch_route_scores(const RouteArgs& a, cudaStream_t s, uint64_t* launches);
 
