@@ -53,6 +53,12 @@ __device__ __forceinline__ float lowest() {
   return TYPE == 0 ? -3.402823466e38f : TYPE == 1 ? -3.389531390e38f : -65504.0f;
 }
 
+// the warp's largest value, NaN aside, in one instruction
+__device__ __forceinline__ float redux_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
 __device__ __forceinline__ double warp_max_d(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(kAll, v, o));
@@ -162,6 +168,15 @@ __device__ __noinline__ void route_scores_64(const RouteArgs& a, long long t, do
   if (lane == 0 && a.mass) a.mass[t] = (float)mass;
 }
 
+// 1 / (1 + exp(-l)) from the approximate power of two and reciprocal: within
+// (2 + 1.173 |l|) + 1.5 ulp; for choices that carry a bound only.
+__device__ __forceinline__ float rough_sigmoid(float l) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(l * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
+
 constexpr int kCand = 64;   // candidates ranked at once
 
 // NV: experts per lane, at least a.chunk.  Lane l holds experts [base, base +
@@ -170,7 +185,7 @@ constexpr int kCand = 64;   // candidates ranked at once
 template <int TYPE, int NV>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_scores_kernel(const __grid_constant__ RouteArgs a) {
   __shared__ int s_id[kRouteWarps][kCand];
-  __shared__ float s_key[kRouteWarps][kCand], s_logit[kRouteWarps][kCand];
+  __shared__ alignas(16) float s_key[kRouteWarps][kCand];
   extern __shared__ double route_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long t = (long long)blockIdx.x * kRouteWarps + warp;
@@ -209,7 +224,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scores_kernel(const __
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    bad |= isnan(l[i]) || l[i] == INFINITY;
+    bad |= !(l[i] < INFINITY);
     if (!(l[i] > lowest<TYPE>())) l[i] = -INFINITY;
     m = fmaxf(m, l[i]);
   }
@@ -224,7 +239,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scores_kernel(const __
     }
     return;
   }
-  m = warp_max(m);
+  m = redux_max(m);
   const bool scored = a.bias != nullptr || (a.pair && a.groups > 1);   // group or picks by scores
   float sum = 1.0f, inv = 1.0f;
   if (!a.sigmoid) {
@@ -234,27 +249,64 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scores_kernel(const __
     sum = warp_sum(sum);
     inv = 1.0f / sum;
   }
-  // How far a choice may be off, S being the token's largest score.  Sigmoid: 2
-  // ulp of the exponential and two roundings, under 3.6e-7 S.  Softmax: the
-  // exponential of a rounded difference d (|d| exp(-|d|) is under 0.37), a sum
-  // of NV + 5 additions whose terms are off by |d| half-ulps each (their mean
-  // |d| is under log E), a reciprocal and a product: under (NV + 40) 6e-8 S.
-  // Adding the bias: under 6e-8 of the choice.
-  const float rel = a.sigmoid ? 4e-7f : (NV + 40) * 6e-8f;
-  float key[NV], kmax = -INFINITY, cabs = 0.0f, smax = 0.0f;
+  // How far a choice may be off, S being the token's largest score.  Sigmoid:
+  // rough_sigmoid's exponential is off by 2 + 1.173 |l| ulp, which counts by
+  // exp(-l) / (1 + exp(-l)), its reciprocal by 1 ulp, the sum by half of one;
+  // s (2 + 1.173 |l|) is largest at the largest logit m for negative ones, and
+  // s |l| / (1 + exp(l)) under 0.28 for positive ones: under
+  // S (6.5e-7 + 1.5e-7 max(-m, 0)).  Softmax: the exponential of a rounded
+  // difference d (|d| exp(-|d|) is under 0.37), a sum of NV + 5 additions whose
+  // terms are off by |d| half-ulps each (their mean |d| is under log E), a
+  // reciprocal and a product: under (NV + 40) 6e-8 S.  Adding the bias: under
+  // 6e-8 of the choice.
+  float key[NV], kmax = -INFINITY, cabs = 0.0f;
+  if (!scored) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    key[i] = l[i];
-    if (scored && l[i] > -INFINITY) {
-      const float s = a.sigmoid ? 1.0f / (1.0f + expf(-l[i])) : expf(l[i] - m) * inv;
-      smax = fmaxf(smax, s);
-      key[i] = a.bias ? s + a.bias[base + i] : s;
-      if (!(fabsf(key[i]) < INFINITY)) key[i] = -INFINITY;   // a bias that is not finite: not available
-      else cabs = fmaxf(cabs, fabsf(key[i]));
+    for (int i = 0; i < NV; ++i) {
+      key[i] = l[i];
+      kmax = fmaxf(kmax, l[i]);
     }
-    kmax = fmaxf(kmax, key[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) key[i] = l[i];
+    if (a.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) key[i] = rough_sigmoid(key[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) key[i] = expf(key[i] - m) * inv;
+    }
+    if (a.bias) {
+      if (a.vec) {
+#pragma unroll
+        for (int i = 0; i < NV; i += 4) {
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (i < count) v = *reinterpret_cast<const float4*>(a.bias + base + i);
+          key[i] += v.x;
+          if (i + 1 < NV) key[i + 1] += v.y;
+          if (i + 2 < NV) key[i + 2] += v.z;
+          if (i + 3 < NV) key[i + 3] += v.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) key[i] += i < count ? a.bias[base + i] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      // masked, or a bias that is not finite: not available
+      const bool there = l[i] > -INFINITY && fabsf(key[i]) < INFINITY;
+      cabs = there ? fmaxf(cabs, fabsf(key[i])) : cabs;
+      key[i] = there ? key[i] : -INFINITY;
+      kmax = fmaxf(kmax, key[i]);
+    }
   }
-  const float bound = scored ? rel * warp_max(smax) + 1.3e-7f * warp_max(cabs) + 1e-37f : 0.0f;
+  float bound = 0.0f;
+  if (scored) {
+    const float rel = a.sigmoid ? 6.5e-7f + 1.5e-7f * fmaxf(-m, 0.0f) : (NV + 40) * 6e-8f;
+    const float most = a.sigmoid ? fminf(1.0f, 1.01f * __expf(m)) : inv;
+    bound = rel * most + 1.3e-7f * redux_max(cabs) + 1e-37f;
+  }
   bool doubt = false;
   if (a.groups > 1) {
     float v1 = kmax, v2 = -INFINITY;
@@ -282,8 +334,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scores_kernel(const __
     const bool kept = rank < a.top_groups && count > 0;
     if (scored) {
       // the worst group kept against the best one left
-      const float in = warp_max(grp < a.groups && rank < a.top_groups ? -value : -INFINITY);
-      const float out = warp_max(grp < a.groups && rank >= a.top_groups ? value : -INFINITY);
+      const float in = redux_max(grp < a.groups && rank < a.top_groups ? -value : -INFINITY);
+      const float out = redux_max(grp < a.groups && rank >= a.top_groups ? value : -INFINITY);
       doubt = !(-in - out > 4.0f * bound + 1.3e-7f * fabsf(out)) && out > -INFINITY;
     }
     if (!kept) {
@@ -334,8 +386,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scores_kernel(const __
     for (int i = 0; i < NV; ++i)
       if (mask >> i & 1) {
         s_id[warp][at] = base + i;
-        s_key[warp][at] = key[i];
-        s_logit[warp][at++] = l[i];
+        s_key[warp][at++] = key[i];
       }
   }
   __syncwarp();
@@ -343,23 +394,21 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scores_kernel(const __
   // then everything in that order.
   const float k0 = lane < n ? s_key[warp][lane] : -INFINITY, k1 = lane + 32 < n ? s_key[warp][lane + 32] : -INFINITY;
   int r0 = 0, r1 = 0;
-  for (int i = 0; i < n; ++i) {
-    const float o = s_key[warp][i];
-    r0 += o > k0 || (o == k0 && i < lane);
-    r1 += o > k1 || (o == k1 && i < lane + 32);
+  for (int i = 0; i < n; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(&s_key[warp][i]);
+    const float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < n) {
+        r0 += i + e < lane ? o[e] >= k0 : o[e] > k0;
+        if (n > 32) r1 += i + e < lane + 32 ? o[e] >= k1 : o[e] > k1;
+      }
   }
   auto place = [&]() {
     const int i0 = lane < n ? s_id[warp][lane] : 0, i1 = lane + 32 < n ? s_id[warp][lane + 32] : 0;
-    const float l0 = lane < n ? s_logit[warp][lane] : 0.0f, l1 = lane + 32 < n ? s_logit[warp][lane + 32] : 0.0f;
     __syncwarp();
-    if (lane < n) {
-      s_id[warp][r0] = i0;
-      s_logit[warp][r0] = l0;
-    }
-    if (lane + 32 < n) {
-      s_id[warp][r1] = i1;
-      s_logit[warp][r1] = l1;
-    }
+    if (lane < n) s_id[warp][r0] = i0;
+    if (lane + 32 < n) s_id[warp][r1] = i1;
   };
   place();
   if (lane < n) s_key[warp][r0] = k0;
@@ -381,7 +430,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scores_kernel(const __
       auto choice = [&](int at, int& id) -> double {
         if (at >= n) return 0.0;
         id = s_id[warp][at];
-        const double x = s_logit[warp][at];
+        const double x = load_logit<TYPE>(a.logits, row + id);
         return (a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - (double)m) / sum64) + (double)a.bias[id];
       };
       int i0 = 0, i1 = 0;
@@ -398,7 +447,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scores_kernel(const __
     }
   }
   const int id = lane < a.k ? s_id[warp][lane] : 0;
-  const float lg = lane < a.k ? s_logit[warp][lane] : 0.0f;
+  const float lg = lane < a.k ? load_logit<TYPE>(a.logits, row + id) : 0.0f;
   float s = 0.0f;
   if (lane < a.k) s = a.sigmoid ? 1.0f / (1.0f + expf(-lg)) : expf(lg - m) / sum;
   const float mass = warp_sum(s);
@@ -444,7 +493,7 @@ cudaError_t launch_route_scores(const RouteArgs& args, cudaStream_t s, uint64_t*
   const int size = a.E / a.groups, per = a.type == 0 ? 4 : 8;
   const size_t es = a.type == 0 ? 4 : 2;
   a.chunk = (size + a.lanes - 1) / a.lanes;
-  a.vec = size == a.chunk * a.lanes && a.chunk % per == 0 &&
+  a.vec = size == a.chunk * a.lanes && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0 && a.chunk % per == 0 &&
           ((reinterpret_cast<uintptr_t>(a.logits) | (a.tokens > 1 ? a.row_stride * es : 0)) & 15) == 0;
   if (launches) *launches += 1;
   if (a.type == 0) return launch_type<0>(a, s);

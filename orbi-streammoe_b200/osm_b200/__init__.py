@@ -36,28 +36,42 @@ _TYPES = {"torch.float32": _lib.OSM_TYPE_F32, "torch.bfloat16": _lib.OSM_TYPE_BF
           "torch.float16": _lib.OSM_TYPE_F16}
 
 
+def _type_name(dtype, _names={}):
+    """str(dtype), remembered: a call's checks cost more than its launch otherwise."""
+    name = _names.get(dtype)
+    if name is None:
+        name = _names.setdefault(dtype, str(dtype))
+    return name
+
+
+def _on(t, device: int) -> bool:
+    return t.is_cuda and t.get_device() == device
+
+
 def _rows(t, length: int, count: int, device: int, what: str):
     """(type code, row stride) of a CUDA tensor of `count` rows or more of
     `length` values, each row contiguous."""
-    code = _TYPES.get(str(t.dtype))
+    code = _TYPES.get(_type_name(t.dtype))
     if code is None:
         raise ValueError(f"{what}: fp32, bf16 or fp16 rows")
-    if t.dim() != 2 or t.shape[1] != length or t.shape[0] < count:
-        raise ValueError(f"{what}: {count} rows of {length} values expected, got {tuple(t.shape)}")
-    if (length > 1 and t.stride(1) != 1) or (count > 1 and t.stride(0) < length):
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != length or shape[0] < count:
+        raise ValueError(f"{what}: {count} rows of {length} values expected, got {tuple(shape)}")
+    step, inner = t.stride()
+    if (length > 1 and inner != 1) or (count > 1 and step < length):
         raise ValueError(f"{what}: rows must be contiguous and must not overlap")
-    if t.device.type != "cuda" or t.device.index != device:
+    if not _on(t, device):
         raise ValueError(f"{what}: not on the context's device")
-    return code, t.stride(0) if count > 1 else 0
+    return code, step if count > 1 else 0
 
 
 def _flat(t, dtype: str, count: int, device: int, what: str):
     """A contiguous CUDA tensor of `count` values or more of one type."""
     if t is None:
         return
-    if str(t.dtype) not in dtype or t.numel() < count or not t.is_contiguous():
+    if _type_name(t.dtype) not in dtype or t.numel() < count or not t.is_contiguous():
         raise ValueError(f"{what}: {count} contiguous values of {dtype} expected")
-    if t.device.type != "cuda" or t.device.index != device:
+    if not _on(t, device):
         raise ValueError(f"{what}: not on the context's device")
 
 
