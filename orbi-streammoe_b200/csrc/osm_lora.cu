@@ -925,6 +925,242 @@ __global__ void __launch_bounds__(kDecWarps * 32) lora_decode_kernel(const __gri
       }
 }
 
+// ---------------------------------------------------------------- decode batches
+
+// v = gain A x in fp32 on CUDA cores, one warp per ROWS rows of a token's
+// adapter: for decode batches, whose tokens seldom share an adapter.
+constexpr int kRowWarps = 4;
+template <int XT, int AT, int ROWS>
+__global__ void __launch_bounds__(kRowWarps * 32) lora_v_rows_kernel(const __grid_constant__ LoraArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int chunks = (a.rank + ROWS - 1) / ROWS;
+  const long long w = (long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  const long long t = w / chunks;
+  const int j0 = (int)(w - t * chunks) * ROWS;
+  if (t >= a.tokens) return;
+  int rank;
+  const int id = adapter_of(a, t, rank);
+  if (j0 >= rank) return;
+  float acc[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) acc[r] = 0.0f;
+  const size_t xr = (size_t)t * a.x_stride, ar = (size_t)id * a.a_stride + (size_t)j0 * a.K;
+#pragma unroll 4
+  for (int k = lane * 8; k < a.K; k += 256) {
+    float x[8];
+    load8<XT>(a.x, xr + k, a.x_vec, x);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (j0 + r >= rank) break;
+      float b[8];
+      load8<AT>(a.a, ar + (size_t)r * a.K + k, a.a_vec, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[r] = fmaf(x[e], b[e], acc[r]);
+    }
+  }
+  const float gain = a.gain ? a.gain[id] : 1.0f;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const float s = warp_sum(acc[r]);
+    if (lane == r && j0 + r < rank) a.v[(size_t)t * a.v_stride + j0 + r] = gain * s;
+  }
+}
+
+// A decode batch: W x on mma.sync, 16 MT rows of W by 8 NT tokens per CTA, the
+// groups of K dealt to its 8 warps.  A group's sum of (q - 8) x and its sum of
+// x are taken exactly as the operands stand (q - 8 in the rows' 16-bit type;
+// fp32 rows as three bf16 planes, which hold all 24 bits) and meet scale and
+// c = bias + 8 scale in fp32, so no operand is rounded and nothing has to be
+// prepared.  For bf16 the left operands are scaled by 2^-10 and 2^-6, so that no
+// sum over a group overflows.  A lane's share of a group is 16 consecutive k of a
+// row of W (two Q4 words) and of a token: the order of k within a matrix step is
+// free as long as both sides agree, so both come straight from memory, each W
+// word as the pairs (q_p, q_p+4).  The warps' sums are added in shared memory in
+// their order, then B_a v in fp32; v comes from the kernel before, which this one
+// waits for only there.
+constexpr int kBatWarps = 8;
+
+template <int XT, int MT, int NT>
+struct BatSmem {
+  static constexpr int PITCH = 16 * MT + 4;
+  static constexpr size_t BYTES = (size_t)kBatWarps * 8 * NT * PITCH * 4;
+};
+
+template <int XT, int AT, int MT, int NT>
+__global__ void __launch_bounds__(kBatWarps * 32, MT == 4 ? 1 : 2)
+    lora_batch_kernel(const __grid_constant__ LoraArgs a) {
+  constexpr int MR = 16 * MT, TOK = 8 * NT, PL = XT == 0 ? 3 : 1, PITCH = BatSmem<XT, MT, NT>::PITCH;
+  constexpr int OT = XT == 2 ? 2 : 1;   // type of the operands
+  extern __shared__ float bat_sum[];    // [warp][token][PITCH]
+  __shared__ int s_id[TOK], s_rank[TOK];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+  const int G = a.K >> 6, row_tiles = (a.N + MR - 1) / MR;
+  const int o0 = (int)(blockIdx.x % row_tiles) * MR;
+  const long long t0 = (long long)(blockIdx.x / row_tiles) * TOK;
+  // without a kernel for v before it this one may start early itself
+  if (!a.adapter) pdl_wait();
+  if (tid < TOK) {
+    int rank = 0, id = -1;
+    if (a.adapter && t0 + tid < a.tokens) id = adapter_of(a, t0 + tid, rank);
+    s_id[tid] = id;
+    s_rank[tid] = rank;
+  }
+  float acc[MT][NT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.0f;
+  const uint32_t ones = XT == 2 ? 0x3C003C00u : 0x3C803C80u;   // 1, or 2^-6 in bf16
+
+  for (int grp = warp; grp < G; grp += kBatWarps) {
+    uint32_t w[MT][2][2];
+    uint16_t sc[MT][2], bi[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const size_t o = (size_t)min(o0 + 16 * m + 8 * h + g, a.N - 1);
+        const uint32_t* p = a.packed + o * (a.K >> 3) + grp * 8 + 2 * q;
+        if (a.w_vec) {
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+          w[m][h][0] = v.x;
+          w[m][h][1] = v.y;
+        } else {
+          w[m][h][0] = __ldg(p);
+          w[m][h][1] = __ldg(p + 1);
+        }
+        sc[m][h] = __ldg(a.scales + o * G + grp);
+        bi[m][h] = __ldg(a.biases + o * G + grp);
+      }
+    // right operands: [n][plane][pair of k]
+    uint32_t xb[NT][PL][8];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const long long t = min(t0 + 8 * n + g, a.tokens - 1);
+      const size_t at = (size_t)t * a.x_stride + (size_t)grp * 64 + 16 * q;
+      if constexpr (XT == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float f[8];
+          load8<0>(a.x, at + 8 * h, a.x_vec, f);
+#pragma unroll
+          for (int pl = 0; pl < 3; ++pl) {
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+              xb[n][pl][4 * h + p] = prmt(__float_as_uint(f[p]), __float_as_uint(f[p + 4]), 0x7632);
+            if (pl < 2)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] -= __uint_as_float(__float_as_uint(f[e]) & 0xFFFF0000u);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[4];
+          const uint16_t* p = static_cast<const uint16_t*>(a.x) + at + 8 * h;
+          if (a.x_vec) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = p[2 * e] | (uint32_t)p[2 * e + 1] << 16;
+          }
+          xb[n][0][4 * h] = prmt(r[0], r[2], 0x5410);
+          xb[n][0][4 * h + 1] = prmt(r[0], r[2], 0x7632);
+          xb[n][0][4 * h + 2] = prmt(r[1], r[3], 0x5410);
+          xb[n][0][4 * h + 3] = prmt(r[1], r[3], 0x7632);
+        }
+      }
+    }
+    float gs[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int pl = PL - 1; pl >= 0; --pl)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          mma16<OT>(d, ones, ones, ones, ones, xb[n][pl][2 * j], xb[n][pl][2 * j + 1]);
+      gs[n][0] = d[0];
+      gs[n][1] = d[1];
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      uint32_t l[2][8];   // left operands: [row half][pair of k]
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t v = w[m][h][e >> 2] >> (4 * (e & 3)) & 0x000F000Fu;
+          if constexpr (XT == 2) l[h][e] = h2u(__hsub2(u2h(v | 0x64006400u), u2h(0x64086408u)));   // 1024 + q - 1032
+          else l[h][e] = bf2_fma(v | 0x43004300u, 0x3A803A80u, 0xBE08BE08u);   // (128 + q) 2^-10 - 136 2^-10
+        }
+      const float up = XT == 2 ? 1.0f : 1024.0f, upc = XT == 2 ? 1.0f : 64.0f;
+      float s[2], c[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float sf = bf16_bits_to_f32(sc[m][h]);
+        s[h] = sf * up;
+        c[h] = fmaf(8.0f, sf, bf16_bits_to_f32(bi[m][h])) * upc;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int pl = PL - 1; pl >= 0; --pl)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma16<OT>(d, l[0][2 * j], l[1][2 * j], l[0][2 * j + 1], l[1][2 * j + 1], xb[n][pl][2 * j],
+                      xb[n][pl][2 * j + 1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[m][n][e] = fmaf(s[e >> 1], d[e], fmaf(c[e >> 1], gs[n][e & 1], acc[m][n][e]));
+      }
+    }
+  }
+  float* mine = bat_sum + (size_t)warp * TOK * PITCH;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        mine[(8 * n + 2 * q + (e & 1)) * PITCH + 16 * m + 8 * (e >> 1) + g] = acc[m][n][e];
+  __syncthreads();
+  if (a.adapter) pdl_wait();   // v is complete from here on
+  const int used = G < kBatWarps ? G : kBatWarps;
+#pragma unroll 2
+  for (int i = tid; i < MR * TOK; i += kBatWarps * 32) {
+    const int r = i % MR, tk = i / MR, o = o0 + r;
+    const long long t = t0 + tk;
+    if (o >= a.N || t >= a.tokens) continue;
+    float y = 0.0f;
+    for (int k = 0; k < used; ++k) y += bat_sum[((size_t)k * TOK + tk) * PITCH + r];
+    const int rank = s_rank[tk];
+    if (rank) {
+      const size_t br = (size_t)s_id[tk] * a.b_stride + (size_t)o * a.rank;
+      const float* v = a.v + (size_t)t * a.v_stride;
+      int j = 0;
+      float z = 0.0f;
+      for (; j + 8 <= rank; j += 8) {
+        float b[8];
+        load8<AT>(a.b, br + j, a.b_vec, b);
+        const float4 v0 = __ldcg(reinterpret_cast<const float4*>(v + j));
+        const float4 v1 = __ldcg(reinterpret_cast<const float4*>(v + j) + 1);
+        z = fmaf(b[3], v0.w, fmaf(b[2], v0.z, fmaf(b[1], v0.y, fmaf(b[0], v0.x, z))));
+        z = fmaf(b[7], v1.w, fmaf(b[6], v1.z, fmaf(b[5], v1.y, fmaf(b[4], v1.x, z))));
+      }
+      for (; j < rank; ++j) z = fmaf(load_val<AT>(a.b, br + j), __ldcg(v + j), z);
+      y += z;
+    }
+    store_val<XT>(a.y, (size_t)t * a.y_stride + o, y);
+  }
+}
+
 // ---------------------------------------------------------------- gemm
 
 // What the prep kernel wrote is read with __ldcg: this kernel starts beside
@@ -1603,6 +1839,16 @@ bool decodes(const LoraArgs& a) {
   return a.tokens <= kDecTokens && (size_t)a.tokens * a.K * 4 <= kDecSmem;
 }
 
+// Up to here a decode batch: no kernel prepares operands.
+constexpr int kBatTokens = 256;
+bool batches(const LoraArgs& a) { return !decodes(a) && a.tokens <= kBatTokens; }
+// Products of v up to which each token reads its adapter by itself; above that
+// tiles of tokens share the reads.
+constexpr double kRowsWork = 16e6;
+bool v_by_rows(const LoraArgs& a) {
+  return (decodes(a) || batches(a)) && (double)a.tokens * a.rank * a.K <= kRowsWork;
+}
+
 // Tokens per tile and CTAs per tile (K and the adapters split over a cluster):
 // the smallest of a plain estimate in clocks.  A stage costs its matrix steps
 // (N / 2 clocks each, 4 per plane of x), what it moves through shared memory at
@@ -1676,9 +1922,33 @@ cudaError_t launch_decode(const LoraArgs& a, cudaStream_t s) {
                     sm, 1, s, a);
 }
 
+// The most rows per CTA that still give every SM one.
+template <int XT, int AT>
+cudaError_t launch_batch(const LoraArgs& a, int sms, cudaStream_t s) {
+  constexpr int NT = XT == 0 ? 2 : 4;
+  const unsigned tt = (unsigned)((a.tokens + 8 * NT - 1) / (8 * NT));
+  auto tiles = [&](int mt) { return (unsigned)((a.N + 16 * mt - 1) / (16 * mt)) * tt; };
+  if (tiles(4) >= (unsigned)sms)
+    return launch_cfg(lora_batch_kernel<XT, AT, 4, NT>, tiles(4), kBatWarps * 32, BatSmem<XT, 4, NT>::BYTES, 1, s, a);
+  if (tiles(2) >= (unsigned)sms)
+    return launch_cfg(lora_batch_kernel<XT, AT, 2, NT>, tiles(2), kBatWarps * 32, BatSmem<XT, 2, NT>::BYTES, 1, s, a);
+  return launch_cfg(lora_batch_kernel<XT, AT, 1, NT>, tiles(1), kBatWarps * 32, BatSmem<XT, 1, NT>::BYTES, 1, s, a);
+}
+
 template <int XT, int AT>
 cudaError_t launch(const LoraArgs& a, int sms, cudaStream_t s, uint64_t* launches) {
-  const bool dec = decodes(a);
+  const bool dec = decodes(a) || batches(a);
+  if (a.adapter && v_by_rows(a)) {
+    auto blocks = [&](int rows) {
+      return (unsigned)((a.tokens * ((a.rank + rows - 1) / rows) + kRowWarps - 1) / kRowWarps);
+    };
+    const cudaError_t e =
+        a.tokens * a.rank <= 1024
+            ? launch_cfg(lora_v_rows_kernel<XT, AT, 1>, blocks(1), kRowWarps * 32, 0, 1, s, a)
+            : launch_cfg(lora_v_rows_kernel<XT, AT, 4>, blocks(4), kRowWarps * 32, 0, 1, s, a);
+    if (e != cudaSuccess) return e;
+    if (launches) *launches += 1;
+  }
   const long long rows = (a.tokens + 15) / 16 * 16;
   const long long row_blocks = dec ? 0 : a.row_threads == 32 ? rows / kPrepWarps : rows;
   const long long prep = a.v_blocks + a.l_blocks + a.w_blocks + row_blocks;
@@ -1695,6 +1965,7 @@ cudaError_t launch(const LoraArgs& a, int sms, cudaStream_t s, uint64_t* launche
     if (launches) *launches += 1;
   }
   if (launches) *launches += 1;
+  if (batches(a)) return launch_batch<XT, AT>(a, sms, s);
   if (dec) {
     if (a.tokens == 1) return launch_decode<XT, AT, 1>(a, s);
     if (a.tokens == 2) return launch_decode<XT, AT, 2>(a, s);
@@ -1719,7 +1990,7 @@ long long block_tokens(const LoraArgs& a) {
 
 // The shape of the launches for a.tokens tokens and the workspace they take.
 size_t shape(LoraArgs& a, int sms, unsigned char* base) {
-  const bool dec = decodes(a);
+  const bool dec = decodes(a) || batches(a);
   size_t off = 0;
   a.w_blocks = 0;
   if (!dec) {
@@ -1745,7 +2016,8 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
     const long long most = a.tokens < a.count ? a.tokens : a.count;
     // v: tiles of 16 tokens in the prep kernel while a tile's adapters are worth
     // blocks of their own, a kernel of its own where a prompt's tokens share them
-    if (a.tokens < 1024) {
+    if (v_by_rows(a)) {
+    } else if (a.tokens < 1024) {
       a.v_slots = (int)(most < 16 ? most : 16);
       a.v_blocks = (int)((a.tokens + 15) / 16 * a.v_slots);
     } else {
@@ -1784,6 +2056,13 @@ cudaError_t set_smem() {
   dec(lora_decode_kernel<XT, AT, 8, 1>);
   dec(lora_decode_kernel<XT, AT, 4, 2>);
   dec(lora_decode_kernel<XT, AT, 8, 2>);
+  constexpr int NT = XT == 0 ? 2 : 4;
+  auto bat = [&](auto kernel, size_t bytes) {
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  };
+  bat(lora_batch_kernel<XT, AT, 1, NT>, BatSmem<XT, 1, NT>::BYTES);
+  bat(lora_batch_kernel<XT, AT, 2, NT>, BatSmem<XT, 2, NT>::BYTES);
+  bat(lora_batch_kernel<XT, AT, 4, NT>, BatSmem<XT, 4, NT>::BYTES);
   return e;
 }
 
