@@ -491,8 +491,9 @@ struct LoraArgs {
   int NT, split;            // tokens per tile, CTAs per tile
   // the prep kernel: blocks for v (tiles of 16 tokens, v_slots blocks per tile
   // for its adapters), for the lists, for W, and threads per row of x; after_v:
-  // blocks of the kernel that computes v instead (tiles of 32)
-  int v_blocks, v_slots, l_blocks, w_blocks, row_threads, after_v;
+  // blocks of the kernel that computes v instead (tiles of 32); v_self: the
+  // decode kernel does
+  int v_blocks, v_slots, l_blocks, w_blocks, row_threads, after_v, v_self;
   int x_vec, w_vec, m_vec, a_vec, b_vec;  // 16-byte aligned rows (m: scales and biases)
 };
 cudaError_t init_lora_attributes(int max_smem);

@@ -804,25 +804,29 @@ __global__ void __launch_bounds__(kPrepThreads, 2) lora_prep_kernel(const __grid
 
 // ---------------------------------------------------------------- few tokens
 
-// Up to 8 tokens: the projection on CUDA cores in fp32, one warp per ROWS rows
+// Up to 4 tokens: the projection on CUDA cores in fp32, one warp per ROWS rows
 // of W and all tokens, lane l the groups l, l + 32, ... of a row.  Bound by
-// latency: a launch reads about 2.4 MB for 2048 x 2048.  It starts beside the
-// kernel that computes v and waits for it only before the adapters' term.
+// latency: a launch reads about 2.4 MB for 2048 x 2048.  v is computed by every
+// block for itself while that reads little (v_self), which spares a launch;
+// otherwise this kernel starts beside the one that computes v and waits for it
+// only before the adapters' term.
 // x is kept in shared memory in fp32; 16-byte piece c of group g sits at piece
 // c ^ (g & 15), so that the lanes of a warp, which read the same piece of 32
 // groups, meet all banks.
 constexpr int kDecWarps = 8;
-constexpr int kDecTokens = 8;
+constexpr int kDecTokens = 4;
+constexpr int kDecSelf = 256;            // tokens by rank of v in shared memory, most
 constexpr size_t kDecSmem = 128 << 10;   // x in shared memory, most
 
 template <int XT, int AT, int TT, int ROWS>
 __global__ void __launch_bounds__(kDecWarps * 32) lora_decode_kernel(const __grid_constant__ LoraArgs a) {
   extern __shared__ float4 dec_x[];   // [token][K / 4]
+  __shared__ float s_v[kDecSelf];     // [token][rank] where this kernel computes v
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int G = a.K >> 6, T = (int)a.tokens;
   const int o0 = ((int)blockIdx.x * kDecWarps + warp) * ROWS;
   // without a kernel for v before it this one may start early itself
-  if (!a.adapter) pdl_wait();
+  if (!a.adapter || a.v_self) pdl_wait();
   for (int i = tid; i < T * G * 8; i += kDecWarps * 32) {
     const int t = i / (G * 8), p = i - t * (G * 8);   // 8 values from 8 p on
     float v[8];
@@ -857,6 +861,29 @@ __global__ void __launch_bounds__(kDecWarps * 32) lora_decode_kernel(const __gri
   };
   if (o0 < a.N && lane < G) load_w(lane);
   __syncthreads();
+  if (a.v_self) {
+    for (int p = warp; p < T * a.rank; p += kDecWarps) {
+      const int t = p / a.rank, j = p - t * a.rank;
+      int rank;
+      const int id = adapter_of(a, t, rank);
+      if (j >= rank) continue;
+      const size_t row = (size_t)id * a.a_stride + (size_t)j * a.K;
+      float s = 0.0f;
+#pragma unroll 8
+      for (int k = lane * 8; k < a.K; k += 256) {
+        float v[8];
+        load8<AT>(a.a, row + k, a.a_vec, v);
+        const int g = k >> 6, c = (k >> 2) & 15;
+        const float4* xg = dec_x + ((size_t)t * G + g) * 16;
+        const float4 x0 = xg[c ^ (g & 15)], x1 = xg[(c + 1) ^ (g & 15)];
+        s = fmaf(v[3], x0.w, fmaf(v[2], x0.z, fmaf(v[1], x0.y, fmaf(v[0], x0.x, s))));
+        s = fmaf(v[7], x1.w, fmaf(v[6], x1.z, fmaf(v[5], x1.y, fmaf(v[4], x1.x, s))));
+      }
+      s = warp_sum(s);
+      if (lane == 0) s_v[p] = (a.gain ? a.gain[id] : 1.0f) * s;
+    }
+    __syncthreads();
+  }
   if (o0 >= a.N) return;
   for (int g = lane; g < G; g += 32) {
     if (g >= 32) load_w(g);
@@ -899,11 +926,11 @@ __global__ void __launch_bounds__(kDecWarps * 32) lora_decode_kernel(const __gri
         b[r][t] = lane < rank[t] && o0 + r < a.N
                       ? load_val<AT>(a.b, (size_t)id[t] * a.b_stride + (size_t)(o0 + r) * a.rank + lane) : 0.0f;
     }
-    pdl_wait();  // v is complete from here on
+    if (!a.v_self) pdl_wait();  // v is complete from here on
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       for (int j = lane; j < rank[t]; j += 32) {
-        const float v = __ldcg(a.v + (size_t)t * a.v_stride + j);
+        const float v = a.v_self ? s_v[t * a.rank + j] : __ldcg(a.v + (size_t)t * a.v_stride + j);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
           const float bv = j == lane ? b[r][t]
@@ -981,6 +1008,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) lora_v_rows_kernel(const __gri
 // their order, then B_a v in fp32; v comes from the kernel before, which this one
 // waits for only there.
 constexpr int kBatWarps = 8;
+constexpr int kBatRank = 256;   // v in shared memory, most
 
 template <int XT, int MT, int NT>
 struct BatSmem {
@@ -993,7 +1021,9 @@ __global__ void __launch_bounds__(kBatWarps * 32, MT == 4 ? 1 : 2)
     lora_batch_kernel(const __grid_constant__ LoraArgs a) {
   constexpr int MR = 16 * MT, TOK = 8 * NT, PL = XT == 0 ? 3 : 1, PITCH = BatSmem<XT, MT, NT>::PITCH;
   constexpr int OT = XT == 2 ? 2 : 1;   // type of the operands
-  extern __shared__ float bat_sum[];    // [warp][token][PITCH]
+  extern __shared__ float4 bat_smem[];
+  float* bat_sum = reinterpret_cast<float*>(bat_smem);                    // [warp][token][PITCH]
+  float* bat_v = bat_sum + BatSmem<XT, MT, NT>::BYTES / 4;                // [token][v_stride]
   __shared__ int s_id[TOK], s_rank[TOK];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
   const int G = a.K >> 6, row_tiles = (a.N + MR - 1) / MR;
@@ -1130,34 +1160,47 @@ __global__ void __launch_bounds__(kBatWarps * 32, MT == 4 ? 1 : 2)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         mine[(8 * n + 2 * q + (e & 1)) * PITCH + 16 * m + 8 * (e >> 1) + g] = acc[m][n][e];
+  if (a.adapter) {
+    __syncthreads();   // s_rank
+    pdl_wait();        // v is complete from here on
+    const int stride = (int)a.v_stride;
+    for (int i = tid * 4; i < TOK * stride; i += kBatWarps * 128) {
+      const int tk = i / stride, j = i - tk * stride;
+      if (j < s_rank[tk])   // what lies behind the rank is not used
+        *reinterpret_cast<float4*>(bat_v + i) = __ldcg(reinterpret_cast<const float4*>(a.v + (size_t)(t0 + tk) * stride + j));
+    }
+  }
   __syncthreads();
-  if (a.adapter) pdl_wait();   // v is complete from here on
   const int used = G < kBatWarps ? G : kBatWarps;
 #pragma unroll 2
   for (int i = tid; i < MR * TOK; i += kBatWarps * 32) {
     const int r = i % MR, tk = i / MR, o = o0 + r;
-    const long long t = t0 + tk;
-    if (o >= a.N || t >= a.tokens) continue;
+    if (o >= a.N || t0 + tk >= a.tokens) continue;
     float y = 0.0f;
-    for (int k = 0; k < used; ++k) y += bat_sum[((size_t)k * TOK + tk) * PITCH + r];
+    if (used == kBatWarps) {
+#pragma unroll
+      for (int k = 0; k < kBatWarps; ++k) y += bat_sum[(k * TOK + tk) * PITCH + r];
+    } else {
+      for (int k = 0; k < used; ++k) y += bat_sum[(k * TOK + tk) * PITCH + r];
+    }
     const int rank = s_rank[tk];
     if (rank) {
       const size_t br = (size_t)s_id[tk] * a.b_stride + (size_t)o * a.rank;
-      const float* v = a.v + (size_t)t * a.v_stride;
-      int j = 0;
+      const float* v = bat_v + tk * (int)a.v_stride;
       float z = 0.0f;
+      int j = 0;
+#pragma unroll 4
       for (; j + 8 <= rank; j += 8) {
         float b[8];
         load8<AT>(a.b, br + j, a.b_vec, b);
-        const float4 v0 = __ldcg(reinterpret_cast<const float4*>(v + j));
-        const float4 v1 = __ldcg(reinterpret_cast<const float4*>(v + j) + 1);
+        const float4 v0 = *reinterpret_cast<const float4*>(v + j), v1 = *reinterpret_cast<const float4*>(v + j + 4);
         z = fmaf(b[3], v0.w, fmaf(b[2], v0.z, fmaf(b[1], v0.y, fmaf(b[0], v0.x, z))));
         z = fmaf(b[7], v1.w, fmaf(b[6], v1.z, fmaf(b[5], v1.y, fmaf(b[4], v1.x, z))));
       }
-      for (; j < rank; ++j) z = fmaf(load_val<AT>(a.b, br + j), __ldcg(v + j), z);
+      for (; j < rank; ++j) z = fmaf(load_val<AT>(a.b, br + j), v[j], z);
       y += z;
     }
-    store_val<XT>(a.y, (size_t)t * a.y_stride + o, y);
+    store_val<XT>(a.y, (size_t)(t0 + tk) * a.y_stride + o, y);
   }
 }
 
@@ -1839,14 +1882,35 @@ bool decodes(const LoraArgs& a) {
   return a.tokens <= kDecTokens && (size_t)a.tokens * a.K * 4 <= kDecSmem;
 }
 
-// Up to here a decode batch: no kernel prepares operands.
+// Rows of W per warp of the decode kernel: more of them share the reads of x
+// from shared memory, fewer leave more warps.
+int dec_rows(const LoraArgs& a) { return a.tokens > 2 && a.N >= 1024 ? 2 : 1; }
+unsigned dec_blocks(const LoraArgs& a) {
+  const int rows = dec_rows(a) * kDecWarps;
+  return (unsigned)((a.N + rows - 1) / rows);
+}
+// Bytes of the adapters that all blocks together may read again for v: about
+// what a launch costs.
+constexpr double kSelfBytes = 8e6;
+bool v_by_self(const LoraArgs& a) {
+  return decodes(a) && a.tokens * a.rank <= kDecSelf &&
+         (double)a.tokens * a.rank * a.K * 2 * dec_blocks(a) <= kSelfBytes;
+}
+// Up to here a decode batch, for which no kernel prepares operands: mma.sync
+// products (three per product for fp32 rows) against operands that cost about
+// 15 us to prepare.  bf16 2048 x 2048: 128 tokens 21 us against 34, 256 tokens
+// 33 against 25; fp16 512 -> 2048, 256 tokens: 18.5 against 37.
 constexpr int kBatTokens = 256;
-bool batches(const LoraArgs& a) { return !decodes(a) && a.tokens <= kBatTokens; }
+constexpr double kBatWork = 1e9;
+bool batches(const LoraArgs& a) {
+  return !decodes(a) && a.tokens <= kBatTokens && (!a.adapter || a.rank <= kBatRank) &&
+         (double)a.tokens * a.N * a.K * (a.x_type == 0 ? 3 : 1) <= kBatWork;
+}
 // Products of v up to which each token reads its adapter by itself; above that
 // tiles of tokens share the reads.
 constexpr double kRowsWork = 16e6;
 bool v_by_rows(const LoraArgs& a) {
-  return (decodes(a) || batches(a)) && (double)a.tokens * a.rank * a.K <= kRowsWork;
+  return (decodes(a) || batches(a)) && !v_by_self(a) && (double)a.tokens * a.rank * a.K <= kRowsWork;
 }
 
 // Tokens per tile and CTAs per tile (K and the adapters split over a cluster):
@@ -1910,29 +1974,28 @@ cudaError_t launch_cfg(K kernel, unsigned grid, unsigned block, size_t smem, int
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-// Rows of W per warp of the decode kernel: more of them share the reads of x
-// from shared memory, fewer leave more warps.
 template <int XT, int AT, int TT>
 cudaError_t launch_decode(const LoraArgs& a, cudaStream_t s) {
   const size_t sm = (size_t)a.tokens * a.K * 4;
-  if (TT >= 4 && a.N >= 1024)
-    return launch_cfg(lora_decode_kernel<XT, AT, TT, 2>, (unsigned)((a.N + 2 * kDecWarps - 1) / (2 * kDecWarps)),
-                      kDecWarps * 32, sm, 1, s, a);
-  return launch_cfg(lora_decode_kernel<XT, AT, TT, 1>, (unsigned)((a.N + kDecWarps - 1) / kDecWarps), kDecWarps * 32,
-                    sm, 1, s, a);
+  if (TT >= 4 && dec_rows(a) == 2)
+    return launch_cfg(lora_decode_kernel<XT, AT, TT, 2>, dec_blocks(a), kDecWarps * 32, sm, 1, s, a);
+  return launch_cfg(lora_decode_kernel<XT, AT, TT, 1>, dec_blocks(a), kDecWarps * 32, sm, 1, s, a);
 }
 
-// The most rows per CTA that still give every SM one.
+// The most rows per CTA that still give every SM one (for 16-bit rows 64 rows
+// leave no room for a second CTA on the SM: 23.4 us against 18.5).
 template <int XT, int AT>
 cudaError_t launch_batch(const LoraArgs& a, int sms, cudaStream_t s) {
   constexpr int NT = XT == 0 ? 2 : 4;
   const unsigned tt = (unsigned)((a.tokens + 8 * NT - 1) / (8 * NT));
+  const size_t v = a.adapter ? (size_t)8 * NT * a.v_stride * 4 : 0;
   auto tiles = [&](int mt) { return (unsigned)((a.N + 16 * mt - 1) / (16 * mt)) * tt; };
-  if (tiles(4) >= (unsigned)sms)
-    return launch_cfg(lora_batch_kernel<XT, AT, 4, NT>, tiles(4), kBatWarps * 32, BatSmem<XT, 4, NT>::BYTES, 1, s, a);
+  if constexpr (XT == 0)
+    if (tiles(4) >= (unsigned)sms)
+      return launch_cfg(lora_batch_kernel<XT, AT, 4, NT>, tiles(4), kBatWarps * 32, BatSmem<XT, 4, NT>::BYTES + v, 1, s, a);
   if (tiles(2) >= (unsigned)sms)
-    return launch_cfg(lora_batch_kernel<XT, AT, 2, NT>, tiles(2), kBatWarps * 32, BatSmem<XT, 2, NT>::BYTES, 1, s, a);
-  return launch_cfg(lora_batch_kernel<XT, AT, 1, NT>, tiles(1), kBatWarps * 32, BatSmem<XT, 1, NT>::BYTES, 1, s, a);
+    return launch_cfg(lora_batch_kernel<XT, AT, 2, NT>, tiles(2), kBatWarps * 32, BatSmem<XT, 2, NT>::BYTES + v, 1, s, a);
+  return launch_cfg(lora_batch_kernel<XT, AT, 1, NT>, tiles(1), kBatWarps * 32, BatSmem<XT, 1, NT>::BYTES + v, 1, s, a);
 }
 
 template <int XT, int AT>
@@ -1969,8 +2032,7 @@ cudaError_t launch(const LoraArgs& a, int sms, cudaStream_t s, uint64_t* launche
   if (dec) {
     if (a.tokens == 1) return launch_decode<XT, AT, 1>(a, s);
     if (a.tokens == 2) return launch_decode<XT, AT, 2>(a, s);
-    if (a.tokens <= 4) return launch_decode<XT, AT, 4>(a, s);
-    return launch_decode<XT, AT, 8>(a, s);
+    return launch_decode<XT, AT, 4>(a, s);
   }
   const long long tiles = (long long)((a.N + kLgM - 1) / kLgM) * ((a.tokens + a.NT - 1) / a.NT);
   const unsigned grid = (unsigned)(a.split > 1 ? tiles * a.split : tiles < sms ? tiles : sms);
@@ -2007,7 +2069,7 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
     a.wbias = reinterpret_cast<uint32_t*>(base + off);
     off += up((size_t)a.w_blocks * (a.x_type == 0 ? 2 : 1) * ((nk + 63) / 64) * 32 * kLgM * 4);
   }
-  a.v_blocks = a.l_blocks = a.after_v = 0;
+  a.v_blocks = a.l_blocks = a.after_v = a.v_self = 0;
   a.v_stride = 0;
   a.v_slots = 1;
   if (a.adapter) {
@@ -2016,7 +2078,9 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
     const long long most = a.tokens < a.count ? a.tokens : a.count;
     // v: tiles of 16 tokens in the prep kernel while a tile's adapters are worth
     // blocks of their own, a kernel of its own where a prompt's tokens share them
-    if (v_by_rows(a)) {
+    a.v_self = v_by_self(a);
+    if (a.v_self || v_by_rows(a)) {
+      // no tiles
     } else if (a.tokens < 1024) {
       a.v_slots = (int)(most < 16 ? most : 16);
       a.v_blocks = (int)((a.tokens + 15) / 16 * a.v_slots);
@@ -2053,16 +2117,14 @@ cudaError_t set_smem() {
   dec(lora_decode_kernel<XT, AT, 1, 1>);
   dec(lora_decode_kernel<XT, AT, 2, 1>);
   dec(lora_decode_kernel<XT, AT, 4, 1>);
-  dec(lora_decode_kernel<XT, AT, 8, 1>);
   dec(lora_decode_kernel<XT, AT, 4, 2>);
-  dec(lora_decode_kernel<XT, AT, 8, 2>);
   constexpr int NT = XT == 0 ? 2 : 4;
   auto bat = [&](auto kernel, size_t bytes) {
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(bytes + 8 * NT * kBatRank * 4));
   };
   bat(lora_batch_kernel<XT, AT, 1, NT>, BatSmem<XT, 1, NT>::BYTES);
   bat(lora_batch_kernel<XT, AT, 2, NT>, BatSmem<XT, 2, NT>::BYTES);
-  bat(lora_batch_kernel<XT, AT, 4, NT>, BatSmem<XT, 4, NT>::BYTES);
+  if constexpr (XT == 0) bat(lora_batch_kernel<XT, AT, 4, NT>, BatSmem<XT, 4, NT>::BYTES);
   return e;
 }
 
