@@ -5,29 +5,35 @@
 // [rank][in], B_a [out][rank] in bf16 or fp16; only the first ranks[a] rows of
 // an adapter count.  Rows are fp32, bf16 or fp16.
 //
-// Two kernels, whatever the number of tokens.
+// Up to 4 tokens: lora_decode_kernel (W x on CUDA cores, v[t] = gain A_a x[t]
+// in every block, then B_a v).  One token 2048 -> 512 of rank 16: 6.9 us a
+// call, of which the launch is the larger part.
 //
-// Up to 8 tokens: lora_prep_kernel (v[t] = gain A_a x[t]) and, beside it,
-// lora_decode_kernel (W x on CUDA cores, then B_a v).
+// Decode batches (up to 256 tokens while the products are fewer than what
+// preparing operands costs): lora_v_rows_kernel and, beside it,
+// lora_batch_kernel on mma.sync.  32 bf16 tokens 2048 x 2048, 32 adapters of
+// rank 16: 10 to 12 us; 256 fp16 tokens 512 -> 2048, 64 adapters of rank up to
+// 32: 18.5 us.
 //
-// More: lora_prep_kernel also writes the rows of x as fp16 operands of the
-// tensor cores, each row scaled by a power of two so that its largest value
-// lies in [2^14, 2^15) (fp32 rows as hi + lo, 22 bits; bf16 and fp16 rows
-// exactly), and the sums of their groups of 64.  lora_gemm_kernel then computes
+// More: lora_prep_kernel writes the rows of x as fp16 operands of the tensor
+// cores, each row scaled by a power of two so that its largest value lies in
+// [2^14, 2^15) (fp32 rows as hi + lo, 22 bits; bf16 and fp16 rows exactly), and
+// the sums of their groups of 64.  lora_gemm_kernel then computes
 // D[128 rows of W][N tokens] on tcgen05.  A weight is scale (q - 8) + (bias + 8
-// scale): the first term is exact in fp16 (8 + 3 bits) and goes to tensor
-// memory, scaled by a power of two per row of W; the second multiplies the
-// group sums in further steps of the same sum.  So are the adapters: for the
-// distinct adapters of the tile, B_a against v with zeros in the tokens of
-// other adapters, in bf16 planes, which have the range for any ratio between
-// W, B, x and v.  A tile of many requests needs no sorting and no second pass
-// over y.
+// scale): the first term is exact in fp16 (8 + 3 bits), scaled by a power of
+// two per row of W; the second multiplies the group sums in further steps of
+// the same sum.  So are the adapters: for the distinct adapters of the tile,
+// B_a against v with zeros in the tokens of other adapters, in bf16 planes,
+// which have the range for any ratio between W, B, x and v.  A tile of many
+// requests needs no sorting and no second pass over y.  v is computed by tf32
+// matrix products (x as hi + lo for fp32 rows), once for every distinct adapter
+// of a tile of tokens, in the prep kernel or, from 1024 tokens on, in
+// lora_v_kernel.  4096 bf16 tokens 2048 x 2048, 8 adapters of rank 16: 78 us
+// (of these v 15, operands 14, products 61 with cold caches); 6001 fp32 tokens,
+// 12 adapters of rank 64: 244 us (55, 28, 186).
 //
-// v is computed by tf32 matrix products (x as hi + lo for fp32 rows), once for
-// every distinct adapter of a tile of tokens.
-//
-// What rounds: fp32 rows hold 22 bits of x (products to about 2^-22) and sum
-// 16 products per step; the tensor core's accumulation drops what lies below
+// What rounds there: fp32 rows hold 22 bits of x (products to about 2^-22) and
+// sum 16 products per step; the tensor core's accumulation drops what lies below
 // the accumulator's last place, so after every 4 K groups (32 steps) the
 // partial sum leaves tensor memory and is added in registers, which keeps the
 // loss under 1e-6.  16-bit rows round v to 16 bits and y once.
@@ -955,7 +961,9 @@ __global__ void __launch_bounds__(kDecWarps * 32) lora_decode_kernel(const __gri
 // ---------------------------------------------------------------- decode batches
 
 // v = gain A x in fp32 on CUDA cores, one warp per ROWS rows of a token's
-// adapter: for decode batches, whose tokens seldom share an adapter.
+// adapter: for decode batches, whose tokens seldom share an adapter.  Bound by
+// latency (32 tokens of rank 16 from 2048: 6.5 us with cold caches, mostly
+// before the batch kernel needs v).
 constexpr int kRowWarps = 4;
 template <int XT, int AT, int ROWS>
 __global__ void __launch_bounds__(kRowWarps * 32) lora_v_rows_kernel(const __grid_constant__ LoraArgs a) {
@@ -1008,7 +1016,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) lora_v_rows_kernel(const __gri
 // their order, then B_a v in fp32; v comes from the kernel before, which this one
 // waits for only there.
 constexpr int kBatWarps = 8;
-constexpr int kBatRank = 256;   // v in shared memory, most
+constexpr int kBatRank = 128;   // v in shared memory, most
 
 template <int XT, int MT, int NT>
 struct BatSmem {
@@ -1221,11 +1229,12 @@ constexpr size_t kLgX = 32768;            // x's part: 256 tokens of one plane o
 constexpr size_t kLgStage = kLgA + kLgX;
 constexpr size_t kLgQTile = (size_t)32 * kLgQPitch;
 
-// Both operands are in shared memory.  With the converted weights in tensor
-// memory instead, stores to it bound the kernel at about 0.6 us per 128 x 64
-// weights, however many warps convert.  What is left for tensor memory are two
-// buffers of 256 tokens' sums, so that a tile's epilogue runs beside the next
-// tile's products.
+// Both operands are in shared memory, which leaves tensor memory to two buffers
+// of 256 tokens' sums, so that a tile's epilogue runs beside the next tile's
+// products.  What bounds the kernel is shared memory: 16384 bf16 tokens 2048 x
+// 2048 take 275 us for the whole call, 213 without adapters and stores of y,
+// 181 without the conversion of the weights; the matrix steps alone would take
+// 64 of them.
 template <bool F32>
 struct LgCfg {
   static constexpr int PL = F32 ? 2 : 1;        // planes of x

@@ -127,6 +127,25 @@ def test_ranks_and_types(torch, ctx, T, rank, half, dtype):
     Case(torch, T, 256, 200, rank=rank, n=5, dtype=dtype, half=half, ranks=rank > 1, seed=rank).check(torch, ctx)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("T,K,N,rank,n", [(1, 4096, 24, 127, 2), (2, 2048, 300, 128, 3), (4, 2048, 40, 100, 3),
+                                          (4, 4096, 64, 128, 2), (5, 64, 1, 1, 1), (20, 512, 64, 127, 3),
+                                          (100, 2048, 48, 128, 5), (128, 1024, 640, 128, 4), (255, 704, 777, 20, 64),
+                                          (256, 2048, 2048, 8, 9)])
+def test_large_ranks_and_batches(torch, ctx, T, K, N, rank, n, dtype):
+    Case(torch, T, K, N, rank=rank, n=n, dtype=dtype, seed=rank, ranks=rank == 20).check(torch, ctx)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("T", [2, 20, 300])
+def test_rows_near_the_largest_value(torch, ctx, T, dtype):
+    """Sums of a group of x, or of (q - 8) x, that pass the range of fp32 while y does not."""
+    c = Case(torch, T, 128, 64, dtype=dtype)
+    c.scales, c.biases = c.scales * 2.0 ** -14, c.biases * 2.0 ** -14
+    c.x.copy_(1e38 + 2e38 * torch.rand(T, 128, device="cuda", generator=torch.Generator("cuda").manual_seed(T)))
+    c.check(torch, ctx, lora=False)
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("T", [1, 12, 31, 200])
 def test_without_adapters(torch, ctx, T, dtype):
