@@ -487,7 +487,7 @@ struct LoraArgs {
   uint32_t* wbias;          // biases as operands [N / 128][stage][32][128]
   float* v;                 // gain A x: [tokens][v_stride], or bf16 [tokens][v_planes][v_stride]
   size_t v_stride;
-  int v_planes;             // 0: fp32
+  int v_planes;             // 0: fp32 (decode and batch kernels)
   int NT, split;            // tokens per tile, CTAs per tile
   // the prep kernel: blocks for v (tiles of 16 tokens, v_slots blocks per tile
   // for its adapters), for the lists, for W, and threads per row of x; after_v:

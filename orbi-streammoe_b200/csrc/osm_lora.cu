@@ -27,7 +27,7 @@
 // which have the range for any ratio between W, B, x and v.  A tile of many
 // requests needs no sorting and no second pass over y.  v is computed by tf32
 // matrix products (x as hi + lo for fp32 rows), once for every distinct adapter
-// of a tile of tokens, in the prep kernel or, from 1024 tokens on, in
+// of a tile of tokens, in the prep kernel or, from 4096 tokens on, in
 // lora_v_kernel.  4096 bf16 tokens 2048 x 2048, 8 adapters of rank 16: 78 us
 // (of these v 15, operands 14, products 61 with cold caches); 6001 fp32 tokens,
 // 12 adapters of rank 64: 244 us (55, 28, 186).
@@ -245,9 +245,9 @@ __device__ __forceinline__ void store_planes(const LoraArgs& a, long long t, int
   }
 }
 
-// Few tokens: tiles of 16, v for the tile's distinct adapters slot, slot +
-// v_slots, ...; the 16 warps split K.  v goes out in fp32 for the decode
-// kernel or as planes for the matrix kernel, [token][plane][v_stride].
+// Below 4096 tokens: tiles of 16, v for the tile's distinct adapters slot, slot
+// + v_slots, ...; the 16 warps split K.  v goes out as planes for the matrix
+// kernel, [token][plane][v_stride].
 template <int XT, int AT>
 __device__ __forceinline__ void prep_v(const LoraArgs& a, int block, float* red, VShared& S) {
   constexpr int TOK = 16, KW = kPrepWarps;
@@ -338,10 +338,7 @@ __device__ __forceinline__ void prep_v(const LoraArgs& a, int block, float* red,
         if (S.id[r] == id && j0 + j < ((rank + 15) & ~15)) {
           s.x = j0 + j < rank ? gain * s.x : 0.0f;
           s.y = j0 + j + 1 < rank ? gain * s.y : 0.0f;
-          if (a.v_planes == 0)
-            *reinterpret_cast<float2*>(a.v + (size_t)(t0 + r) * a.v_stride + j0 + j) = s;
-          else
-            store_planes(a, t0 + r, j0 + j, s.x, s.y, row_exponent(m));
+          store_planes(a, t0 + r, j0 + j, s.x, s.y, row_exponent(m));
         }
       }
       __syncthreads();
@@ -810,7 +807,8 @@ __global__ void __launch_bounds__(kPrepThreads, 2) lora_prep_kernel(const __grid
 
 // ---------------------------------------------------------------- few tokens
 
-// Up to 4 tokens: the projection on CUDA cores in fp32, one warp per ROWS rows
+// Up to 4 tokens (8 took 19.5 us here and 13.5 on mma.sync, 2048 x 2048): the
+// projection on CUDA cores in fp32, one warp per ROWS rows
 // of W and all tokens, lane l the groups l, l + 32, ... of a row.  Bound by
 // latency: a launch reads about 2.4 MB for 2048 x 2048.  v is computed by every
 // block for itself while that reads little (v_self), which spares a launch;
@@ -963,7 +961,10 @@ __global__ void __launch_bounds__(kDecWarps * 32) lora_decode_kernel(const __gri
 // v = gain A x in fp32 on CUDA cores, one warp per ROWS rows of a token's
 // adapter: for decode batches, whose tokens seldom share an adapter.  Bound by
 // latency (32 tokens of rank 16 from 2048: 6.5 us with cold caches, mostly
-// before the batch kernel needs v).
+// before the batch kernel needs v).  Tiles of 16 tokens that share the reads of
+// their adapters were slower throughout: whole calls of 128 bf16 tokens 4096 ->
+// 512 with 4 adapters of rank 128 took 57 us against 36, with 128 adapters 64
+// against 51; 128 tokens 2048 -> 512 with 8 of rank 64 took 21 against 20.
 constexpr int kRowWarps = 4;
 template <int XT, int AT, int ROWS>
 __global__ void __launch_bounds__(kRowWarps * 32) lora_v_rows_kernel(const __grid_constant__ LoraArgs a) {
@@ -1899,7 +1900,8 @@ unsigned dec_blocks(const LoraArgs& a) {
   return (unsigned)((a.N + rows - 1) / rows);
 }
 // Bytes of the adapters that all blocks together may read again for v: about
-// what a launch costs.
+// what a launch costs.  One fp32 token 2048 -> 512 of rank 16 (4 MB): 9.1 us in
+// one launch, 11.4 in two; four tokens 2048 x 2048 (32 MB): 22.8 against 11.8.
 constexpr double kSelfBytes = 8e6;
 bool v_by_self(const LoraArgs& a) {
   return decodes(a) && a.tokens * a.rank <= kDecSelf &&
@@ -1915,12 +1917,7 @@ bool batches(const LoraArgs& a) {
   return !decodes(a) && a.tokens <= kBatTokens && (!a.adapter || a.rank <= kBatRank) &&
          (double)a.tokens * a.N * a.K * (a.x_type == 0 ? 3 : 1) <= kBatWork;
 }
-// Products of v up to which each token reads its adapter by itself; above that
-// tiles of tokens share the reads.
-constexpr double kRowsWork = 16e6;
-bool v_by_rows(const LoraArgs& a) {
-  return (decodes(a) || batches(a)) && !v_by_self(a) && (double)a.tokens * a.rank * a.K <= kRowsWork;
-}
+bool v_by_rows(const LoraArgs& a) { return (decodes(a) || batches(a)) && !v_by_self(a); }
 
 // Tokens per tile and CTAs per tile (K and the adapters split over a cluster):
 // the smallest of a plain estimate in clocks.  A stage costs its matrix steps
@@ -2087,10 +2084,15 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
     const long long most = a.tokens < a.count ? a.tokens : a.count;
     // v: tiles of 16 tokens in the prep kernel while a tile's adapters are worth
     // blocks of their own, a kernel of its own where a prompt's tokens share them
+    // (2500 bf16 tokens 2048 x 2048, 8 adapters of rank 16: 72 us against 75; 3500,
+    // every token another of 64: 235 against 329; 3500 fp32 tokens 2048 -> 768, 8
+    // adapters of rank 64: 103 against 102; above, prompts decide: 4096 tokens of 8
+    // requests 85 against 78, 6000 fp32 tokens of 12 of rank 64 255 against 238,
+    // though 6000 tokens that each take another of 64 would gain, 387 against 554)
     a.v_self = v_by_self(a);
     if (a.v_self || v_by_rows(a)) {
       // no tiles
-    } else if (a.tokens < 1024) {
+    } else if (a.tokens < 4096) {
       a.v_slots = (int)(most < 16 ? most : 16);
       a.v_blocks = (int)((a.tokens + 15) / 16 * a.v_slots);
     } else {

@@ -155,7 +155,8 @@ def test_without_adapters(torch, ctx, T, dtype):
     c.check(torch, ctx)
 
 
-@pytest.mark.parametrize("T,n,runs", [(512, 40, None), (300, 300, None), (1000, 3, 125), (1024, 7, 200), (2100, 64, 33)])
+@pytest.mark.parametrize("T,n,runs", [(512, 40, None), (300, 300, None), (1000, 3, 125), (1024, 7, 200), (2100, 64, 33), (4100, 9, 700),
+                                      (4111, 40, 17)])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_many_tokens_and_adapters(torch, ctx, T, n, runs, dtype):
     Case(torch, T, 512, 384, n=n, rank=16, dtype=dtype, runs=runs).check(torch, ctx)
