@@ -1243,6 +1243,13 @@ struct LgCfg {
   static constexpr int GROUP = F32 ? 4 : 1 << 30;  // stages per partial sum
   static constexpr int NV = F32 ? 3 : 2;        // bf16 planes of v
 };
+// Stages that a block of adapters takes in a tile of `tokens`: the nv planes of
+// v, as many a stage as fit beside each other, and for fp16 adapters (`lo`) those
+// that the lo part of B meets, all but the last.
+__host__ __device__ constexpr int lora_passes(int nv, int tokens, bool lo) {
+  const int per = 256 / tokens < nv ? 256 / tokens : nv;
+  return (nv + per - 1) / per + (lo ? (nv - 1 + per - 1) / per : 0);
+}
 // A converter warp's first block of adapters in a tile, brought ahead: the
 // pieces, and the entries of its threads' tokens.
 struct alignas(16) LgAhead {
@@ -1380,15 +1387,14 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
   const uint32_t tmem = S.tmem;
   auto tokens_of = [&](int tile) { return (int)min((long long)a.NT, a.tokens - (long long)(tile / mt) * a.NT); };
   // The adapters' stages: blocks of 64 columns, this CTA's share of them, each
-  // in passes over B's parts (fp16 adapters: hi, lo) and as many planes of v as
-  // a stage holds.
-  constexpr int BPARTS = AT == 2 ? 2 : 1;
+  // in the passes of lora_passes: every stage has matrix steps (a partial sum
+  // that began with a stage without any would hold what its buffer held before).
+  constexpr bool BLO = AT == 2;
   auto v_planes = [&](int npad) { return min(C::NV, 256 / npad); };
-  auto v_passes = [&](int npad) { const int p = v_planes(npad); return (C::NV + p - 1) / p; };
   auto pieces_at = [&](int tile) { return a.adapter && tile < tiles ? __ldcg(a.n_gran + tile / mt) : 0; };
   auto stages_of = [&](int npad, int ng) {
     const int nb = (ng + 3) >> 2;
-    return nkm + (nb > rank_c ? (nb - rank_c + split - 1) / split * BPARTS * v_passes(npad) : 0);
+    return nkm + (nb > rank_c ? (nb - rank_c + split - 1) / split * lora_passes(C::NV, npad, BLO) : 0);
   };
 
   if (warp == 0) {
@@ -1440,7 +1446,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
       for (int tile = first_tile; tile < tiles && ok; tile += step) {
         const int npad = (tokens_of(tile) + 15) & ~15;
         const uint32_t idf = idesc16(kLgM, npad, false), idb = idesc16(kLgM, npad, true);
-        const int vpl = v_planes(npad), vps = v_passes(npad);
+        const int vpl = v_planes(npad), hi = lora_passes(C::NV, npad, false), passes = lora_passes(C::NV, npad, BLO);
         const int total = stages_of(npad, ng);
         ng = pieces_at(tile + step);
         for (int c = 0; c < total; ++c, ++os) {
@@ -1469,9 +1475,10 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
             // the lo part of x; not for the lo part of the biases
             if (F32 && (k_lo + c < nk || ((k_lo + c - nk) & 1) == 0)) issue((uint32_t)C::NMAX * 128, idf);
           } else {
-            const int pass = (c - nkm) % (BPARTS * vps), p0 = pass % vps * vpl;
-            // the lo part of B meets all but the last plane of v
-            const int planes = min(pass >= vps ? C::NV - 1 : C::NV, p0 + vpl) - p0;
+            const int pass = (c - nkm) % passes;
+            const bool lo_part = pass >= hi;
+            const int p0 = (lo_part ? pass - hi : pass) * vpl;
+            const int planes = min(lo_part ? C::NV - 1 : C::NV, p0 + vpl) - p0;
             for (int p = 0; p < planes; ++p) issue((uint32_t)(p * npad * 128), idb);
           }
           commit(&S.opempty[st]);
@@ -1602,7 +1609,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
         return true;
       };
       // ---- a stage of adapters: a block of 64 columns, four pieces of 16 rows ----
-      const int vpl = v_planes(npad), vps = v_passes(npad), passes = BPARTS * vps;
+      const int vpl = v_planes(npad), hi = lora_passes(C::NV, npad, false), passes = lora_passes(C::NV, npad, BLO);
       auto block_of = [&](int c) { return rank_c + (c - nkm) / passes * split; };
       const int c_first = nkm + ((nkm ^ grp) & 1);   // this group's first such stage
       LgAhead& ahead = S.ahead[warp - 2];
@@ -1626,8 +1633,10 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
       auto adapters = [&](int c) -> bool {
         const uint32_t oc = os + (uint32_t)c;
         const int st = (int)(oc % kLgRO);
-        const int blk = block_of(c), pass = (c - nkm) % passes, p0 = pass % vps * vpl;
-        const bool lo_part = pass >= vps;
+        const int blk = block_of(c), pass = (c - nkm) % passes;
+        const bool lo_part = pass >= hi;
+        const int p0 = (lo_part ? pass - hi : pass) * vpl;
+        const int planes = min(lo_part ? C::NV - 1 : C::NV, p0 + vpl) - p0;
         const bool here = c == c_first;
         if (here) {
           asm volatile("cp.async.wait_all;" ::: "memory");
@@ -1673,7 +1682,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
           const uint16_t* v = reinterpret_cast<const uint16_t*>(a.v) +
                               ((size_t)(tn + n) * C::NV + p0) * a.v_stride - q0 * 16;
           unsigned char* at = stages + (size_t)st * kLgStage + kLgA + (size_t)n * 128;
-          for (int p = 0; p < vpl && p0 + p < C::NV; ++p) {
+          for (int p = 0; p < planes; ++p) {
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
               const bool in = (u >> 1) >= q0 && (u >> 1) < q1;
@@ -1937,9 +1946,9 @@ void lg_shape(const LoraArgs& a, int sms, int* NT, int* split) {
     const long long tiles = mt * ((a.tokens + n - 1) / n);
     double lora = 0.0;
     if (a.adapter) {
-      const int nv = f32 ? 3 : 2, per = 256 / n < nv ? 256 / n : nv, passes = (nv + per - 1) / per;
+      const int passes = lora_passes(f32 ? 3 : 2, n, a.a_type == 2);
       const double many = a.tokens <= 512 ? (a.count < n ? a.count : n) : 2.0;
-      lora = (a.a_type == 2 ? 2 : 1) * passes * (many * ((a.rank + 15) / 16) / 4.0 + 0.5);
+      lora = passes * (many * ((a.rank + 15) / 16) / 4.0 + 0.5);
     }
     for (int s = 1; s <= 8; s *= 2) {
       if (s > nk || (s > 1 && tiles * s > (s == 8 ? 128 : sms))) break;
