@@ -18,11 +18,13 @@
 // More: lora_prep_kernel writes the rows of x as fp16 operands of the tensor
 // cores, each row scaled by a power of two so that its largest value lies in
 // [2^14, 2^15) (fp32 rows as hi + lo, 22 bits; bf16 and fp16 rows exactly), and
-// the sums of their groups of 64.  lora_gemm_kernel then computes
+// the sums of their groups of 64 as hi + lo.  lora_gemm_kernel then computes
 // D[128 rows of W][N tokens] on tcgen05.  A weight is scale (q - 8) + (bias + 8
 // scale): the first term is exact in fp16 (8 + 3 bits), scaled by a power of
-// two per row of W; the second multiplies the group sums in further steps of
-// the same sum.  So are the adapters: for the distinct adapters of the tile,
+// two per row of W; the second, as hi + lo too, multiplies the group sums in
+// further steps of the same sum (the two terms nearly cancel where the weights of
+// a row are of one sign, so neither may have fewer bits than the sum).  So are
+// the adapters: for the distinct adapters of the tile,
 // B_a against v with zeros in the tokens of other adapters, in bf16 planes,
 // which have the range for any ratio between W, B, x and v.  A tile of many
 // requests needs no sorting and no second pass over y.  v is computed by tf32
@@ -36,7 +38,11 @@
 // sum 16 products per step; the tensor core's accumulation drops what lies below
 // the accumulator's last place, so after every 4 K groups (32 steps) the
 // partial sum leaves tensor memory and is added in registers, which keeps the
-// loss under 1e-6.  16-bit rows round v to 16 bits and y once.
+// loss under 1e-6.  16-bit rows keep one sum in tensor memory (the epilogue has
+// no registers for those of 256 tokens), of which a step loses less than 2^-23,
+// and hold v in 16 bits: within 2^-17 of the adapters' term, a 32nd of what
+// rounding an fp16 y of that size does, where a third plane of v would cost
+// every block of adapters another stage.  y is rounded once.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -98,6 +104,12 @@ __device__ __forceinline__ void load8(const void* p, size_t i, bool vec, float (
     for (int e = 0; e < 8; ++e) v[e] = load_val<TYPE>(p, i + e);
   }
 }
+
+// Chunks of 64 columns that the groups' sums and the biases take behind K's nk
+// groups.  fp32 rows: a column per group, hi and lo in planes of their own.
+// 16-bit rows: three columns per group, (c hi, sum hi), (c hi, sum lo), (c lo,
+// sum hi), so that one plane holds them.
+__host__ __device__ constexpr int bias_chunks(int nk, bool f32) { return ((f32 ? nk : 3 * nk) + 63) / 64; }
 
 // Exponent e of a row whose largest magnitude is m: m 2^-e lies in
 // [2^14, 2^15); 0 for a zero row.  Not below -100, so that 2^-e and what it
@@ -579,7 +591,7 @@ __device__ __forceinline__ void prep_row(const LoraArgs& a, long long t) {
   const int lane = threadIdx.x % TPR;
   const bool live = t < a.tokens;
   const size_t row = (size_t)t * a.x_stride;
-  const int row_in = (int)(t % a.NT), nk = a.K >> 6, nkp = nk + (nk + 63) / 64;
+  const int row_in = (int)(t % a.NT), nk = a.K >> 6, nkp = nk + bias_chunks(nk, XT == 0);
   unsigned char* tile = a.planes + (size_t)(t / a.NT) * nkp * PB * a.NT * 128 + (size_t)row_in * 128;
   float kept[KEEP][8];
   float m = 0.0f;
@@ -619,6 +631,8 @@ __device__ __forceinline__ void prep_row(const LoraArgs& a, long long t) {
   auto chunk_at = [&](int k, int unit) {
     return tile + (size_t)k * PB * a.NT * 128 + ((unit ^ (row_in & 7)) << 4);
   };
+  // column c of the groups' sums
+  auto column_at = [&](int c) { return chunk_at(nk + (c >> 6), (c & 63) >> 3) + (c & 7) * 2; };
   // the 8 values from i on and, by 8 threads together, their group's sum
   auto put = [&](int i, const float (&v)[8]) {
     uint32_t hi[4], lo[4];
@@ -643,12 +657,18 @@ __device__ __forceinline__ void prep_row(const LoraArgs& a, long long t) {
     sum += __shfl_xor_sync(mask, sum, 2);
     sum += __shfl_xor_sync(mask, sum, 4);
     if ((threadIdx.x & 7) == 0) {
-      const int grp = i >> 6, col = grp & 63;
+      const int grp = i >> 6;
       const float x = sum * (1.0f / 64.0f);  // stays below 2^15; the biases carry the 64
-      const __half h = __float2half_rn(x);
-      unsigned char* gat = chunk_at(nk + (grp >> 6), col >> 3) + (col & 7) * 2;
-      *reinterpret_cast<__half*>(gat) = h;
-      if constexpr (PB == 2) *reinterpret_cast<__half*>(gat + (size_t)a.NT * 128) = __float2half_rn(x - __half2float(h));
+      const __half h = __float2half_rn(x), l = __float2half_rn(x - __half2float(h));
+      if constexpr (PB == 2) {
+        unsigned char* gat = column_at(grp);
+        *reinterpret_cast<__half*>(gat) = h;
+        *reinterpret_cast<__half*>(gat + (size_t)a.NT * 128) = l;
+      } else {
+        *reinterpret_cast<__half*>(column_at(3 * grp)) = h;
+        *reinterpret_cast<__half*>(column_at(3 * grp + 1)) = l;
+        *reinterpret_cast<__half*>(column_at(3 * grp + 2)) = h;
+      }
     }
   };
 #pragma unroll
@@ -663,8 +683,8 @@ __device__ __forceinline__ void prep_row(const LoraArgs& a, long long t) {
     put(i, v);
   }
   // zeros behind the last group's sum
-  for (int c = nk + lane; c < (nkp - nk) * 64; c += TPR) {
-    unsigned char* at = chunk_at(nk + (c >> 6), (c & 63) >> 3) + (c & 7) * 2;
+  for (int c = (PB == 2 ? nk : 3 * nk) + lane; c < (nkp - nk) * 64; c += TPR) {
+    unsigned char* at = column_at(c);
     *reinterpret_cast<__half*>(at) = __float2half_rn(0.0f);
     if constexpr (PB == 2) *reinterpret_cast<__half*>(at + (size_t)a.NT * 128) = __float2half_rn(0.0f);
   }
@@ -676,13 +696,15 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int i);
 // The exponents of 128 rows of W and their biases as operands.  A weight is
 // scale (q - 8) + c with c = bias + 8 scale; the exponent is that of the largest
 // of 16 |scale|, which keeps the converters' 24 scale in range, and 64 |c| (the
-// groups' sums of x are kept as 1/64, so c carries the 64).  Operands [stage][pair of groups][row]: fp16 pairs, hi, and for fp32
-// rows of x lo in a stage of its own.  Four threads per row.
+// groups' sums of x are kept as 1/64, so c carries the 64).  Operands
+// [stage][pair of columns][row], fp16 pairs: for fp32 rows of x a column per
+// group, hi, and lo in a stage of its own; else the three columns per group of
+// bias_chunks.  Four threads per row.
 template <bool F32>
 __device__ __forceinline__ void prep_weights(const LoraArgs& a, int tile) {
   constexpr int PARTS = kPrepThreads / 128;
   const int row = threadIdx.x / PARTS, part = threadIdx.x % PARTS, o = tile * 128 + row;
-  const int nk = a.K >> 6, n8 = (nk + 7) / 8, nbk = (nk + 63) / 64;
+  const int nk = a.K >> 6, n8 = (nk + 7) / 8, nbk = bias_chunks(nk, F32);
   auto mid = [](float s, float b) { return 64.0f * fmaf(8.0f, s, b); };
   float m = 0.0f;
   if (o < a.N) {
@@ -704,24 +726,30 @@ __device__ __forceinline__ void prep_weights(const LoraArgs& a, int tile) {
   const float sc = pow2(-ew);
   uint32_t* out = a.wbias + (size_t)tile * (F32 ? 2 : 1) * nbk * 32 * 128 + row;
 #pragma unroll 4
-  for (int k8 = part; k8 < nbk * 8; k8 += PARTS) {
+  for (int k8 = part; k8 < (F32 ? nbk * 8 : (nbk * 32 + 11) / 12); k8 += PARTS) {
     uint4 sv = make_uint4(0, 0, 0, 0), bv = sv;
     if (o < a.N && k8 < n8) {
       sv = load_meta(a, a.scales, o, k8);
       bv = load_meta(a, a.biases, o, k8);
     }
-    const int bi = k8 >> 3, col = (k8 & 7) * 4;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       const uint32_t sw = word_of(sv, p), bw = word_of(bv, p);
       const float f0 = mid(bf_lo(sw), bf_lo(bw)) * sc, f1 = mid(bf_hi(sw), bf_hi(bw)) * sc;
       const __half2 h = __floats2half2_rn(f0, f1);
+      const float2 f = __half22float2(h);
+      const uint32_t hw = h2u(h), lw = h2u(__floats2half2_rn(f0 - f.x, f1 - f.y));
       if constexpr (F32) {
-        const float2 f = __half22float2(h);
-        out[(size_t)((bi * 2) * 32 + col + p) * 128] = h2u(h);
-        out[(size_t)((bi * 2 + 1) * 32 + col + p) * 128] = h2u(__floats2half2_rn(f0 - f.x, f1 - f.y));
+        const int bi = k8 >> 3, col = (k8 & 7) * 4;
+        out[(size_t)((bi * 2) * 32 + col + p) * 128] = hw;
+        out[(size_t)((bi * 2 + 1) * 32 + col + p) * 128] = lw;
       } else {
-        out[(size_t)(bi * 32 + col + p) * 128] = h2u(h);
+        // two groups, six columns: hi0 hi0 | lo0 hi1 | hi1 lo1
+        const uint32_t w[3] = {prmt(hw, hw, 0x1010), prmt(lw, hw, 0x7610), prmt(hw, lw, 0x7632)};
+        const int at = k8 * 12 + p * 3;
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (at + e < nbk * 32) out[(size_t)(at + e) * 128] = w[e];
       }
     }
   }
@@ -1359,8 +1387,8 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
   const int first_tile = split > 1 ? (int)blockIdx.x / split : (int)blockIdx.x;
   const int step = split > 1 ? tiles : (int)gridDim.x;  // a cluster has one tile
   // K in stages: nk groups of 64, then the groups' sums against the biases, 64
-  // groups a stage (fp32 rows: the biases' hi and lo parts in two stages)
-  const int nk = a.K >> 6, nbk = (nk + 63) >> 6, nkv = nk + (F32 ? 2 : 1) * nbk;
+  // columns a stage (fp32 rows: the biases' hi and lo parts in two stages)
+  const int nk = a.K >> 6, nbk = bias_chunks(nk, F32), nkv = nk + (F32 ? 2 : 1) * nbk;
   const int k_lo = nkv * rank_c / split, nkm = nkv * (rank_c + 1) / split - k_lo;
   const int nq = max(0, min(nk - k_lo, nkm));   // of them from Q4 rows
   volatile int* abort = &S.abort;
@@ -1596,7 +1624,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
               av[4 * w + p] = h2u(__hfma2(u2h((v[p] & 0x03C003C0u) | 0x4C004C00u), s2, m24));
           }
         } else {
-          // the biases of 64 groups
+          // 64 columns of biases
           const uint32_t* b =
               a.wbias + ((size_t)(o >> 7) * (nkv - nk) + (size_t)(k_lo + c - nk)) * 32 * 128 + (row & 127);
 #pragma unroll
@@ -2074,7 +2102,8 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
     lg_shape(a, sms, &a.NT, &a.split);
     const long long tiles = (a.tokens + a.NT - 1) / a.NT, nk = a.K >> 6;
     a.planes = base;
-    off += up((size_t)tiles * a.NT * (nk + (nk + 63) / 64) * 128 * (a.x_type == 0 ? 2 : 1));
+    const int nbk = bias_chunks((int)nk, a.x_type == 0);
+    off += up((size_t)tiles * a.NT * (nk + nbk) * 128 * (a.x_type == 0 ? 2 : 1));
     a.ex = reinterpret_cast<int*>(base + off);
     off += up((size_t)((a.tokens + 15) / 16 * 16) * 4);
     a.row_threads = a.tokens >= 1024 ? 32 : kPrepThreads;
@@ -2082,7 +2111,7 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
     a.ew = reinterpret_cast<int*>(base + off);
     off += up((size_t)a.w_blocks * kLgM * 4);
     a.wbias = reinterpret_cast<uint32_t*>(base + off);
-    off += up((size_t)a.w_blocks * (a.x_type == 0 ? 2 : 1) * ((nk + 63) / 64) * 32 * kLgM * 4);
+    off += up((size_t)a.w_blocks * (a.x_type == 0 ? 2 : 1) * nbk * 32 * kLgM * 4);
   }
   a.v_blocks = a.l_blocks = a.after_v = a.v_self = 0;
   a.v_stride = 0;

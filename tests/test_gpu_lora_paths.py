@@ -19,3 +19,52 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("rank,n", [(16, 4), (40, 7)])
 def test_fp32_rows_with_fp16_adapters(torch, ctx, T, K, N, rank, n):  # noqa: F811
     Case(torch, T, K, N, rank=rank, n=n, dtype="fp32", half="fp16").check(torch, ctx)
+
+
+def one_sided(torch, T, K, N, dtype, kind, seed=0):
+    """Weights whose part scale (q - 8) and whose part bias + 8 scale nearly
+    cancel (codes mostly 0 without a bias, or mostly 15 with -15 scale), and rows
+    of x with a mean, so that y is small beside the two."""
+    c = Case(torch, T, K, N, dtype=dtype, seed=seed)
+    g = torch.Generator(device="cuda").manual_seed(seed + T)
+    f = dict(device="cuda", generator=g)
+    if kind != "middle":
+        few = torch.rand(N, K, **f) < 0.02
+        q = torch.where(few, torch.randint(0, 16, (N, K), **f), 0 if kind == "low" else 15)
+        word = torch.zeros(N, K // 8, dtype=torch.int64, device="cuda")
+        for i in range(8):
+            word |= q[:, i::8] << (4 * i)
+        c.packed = torch.where(word >= 2**31, word - 2**32, word).int()
+        c.biases = (0.0 if kind == "low" else -15.0) * c.scales
+    c.x.copy_(1 + 0.25 * torch.randn(T, K, **f))
+    return c
+
+
+@pytest.mark.parametrize("kind", ["low", "high", "middle"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("T,K,N", [(3, 512, 96), (40, 512, 96), (300, 512, 96), (300, 1408, 2048), (1100, 64, 200),
+                                   (4200, 2048, 130)])
+def test_parts_that_cancel(torch, ctx, T, K, N, dtype, kind):  # noqa: F811
+    """No operand of the two parts has fewer than 22 bits, whatever the rows'
+    type: the tolerance of test_gpu_lora without its term 2^-11 C.
+
+    Per group: c = bias + 8 scale is hi + lo of fp16, within 2^-24 of itself; the
+    sum of x is taken in fp32 (10 half-ulps, 2^-24 each, of the sum of magnitudes)
+    and held as hi + lo, 2^-24; the product of the two lo parts is left out, 2^-24:
+    under 16 2^-23 C together.  Steps of 16: K / 16 of the products, 3 K / 1024 of
+    the biases' columns, rounded up to a stage of 4: under K / 8 + K / 256 + 4, each
+    with a loss of 2^-23 of the sum of magnitudes at most.  v is held in 16 bits for
+    16-bit rows, 2^-15 L as there; y of fp16 is rounded to a multiple of 2^-24 at
+    the least."""
+    c = one_sided(torch, T, K, N, dtype, kind, seed=K)
+    c.run(ctx)
+    torch.cuda.synchronize()
+    y, (S, C), L = c.reference(torch)
+    tol = (torch.finfo(c.dt).eps / 2 * y.abs() + (K / 8 + K / 256 + 20) * 2.0 ** -23 * (S + L) + c.rank * 2.0 ** -23 * L
+           + 1e-30)
+    if dtype != "fp32":
+        tol = tol + 2.0 ** -15 * L
+    if dtype == "fp16":
+        tol = tol + 2.0 ** -25
+    off = (c.y.double() - y).abs() / tol
+    assert float(off.max()) <= 1.0, float(off.max())
