@@ -75,6 +75,18 @@ def _flat(t, dtype: str, count: int, device: int, what: str):
         raise ValueError(f"{what}: not on the context's device")
 
 
+_Q4_WORDS = frozenset(("torch.int32", "torch.uint32", "torch.uint8"))
+_Q4_SCALES = frozenset(("torch.bfloat16", "torch.uint16", "torch.int16", "torch.uint8"))
+
+
+def _q4_table(t, types, size: int, device: int, what: str):
+    """A contiguous CUDA tensor of `size` bytes or more in one of `types`."""
+    if _type_name(t.dtype) not in types or t.nbytes < size or not t.is_contiguous():
+        raise ValueError(f"{what}: {size} contiguous bytes in one of {sorted(types)} expected")
+    if not _on(t, device):
+        raise ValueError(f"{what}: not on the context's device")
+
+
 class Routing:
     """How experts are chosen from router logits (osm_routing): softmax or
     sigmoid scores, a bias on the choice alone, groups, top-k, renormalised
@@ -235,7 +247,11 @@ class Context:
                      lora: "Lora | None" = None, adapter=None):
         """y[t] = W x[t] + scale[a] B_a (A_a x[t]) for the adapter a = adapter[t]
         (int32, negative: none) of the table `lora`; x and y rows of one type
-        (fp32, bf16 or fp16), which may be strided."""
+        (fp32, bf16 or fp16), which may be strided.  W: words (or bytes) of eight
+        nibbles, scales and biases in bf16 (or its bits) per group of 64."""
+        _q4_table(packed, _Q4_WORDS, out_dim * in_dim // 2, self.device, "q4_gemv_lora packed")
+        _q4_table(scales_bf16, _Q4_SCALES, out_dim * (in_dim // 64) * 2, self.device, "q4_gemv_lora scales")
+        _q4_table(biases_bf16, _Q4_SCALES, out_dim * (in_dim // 64) * 2, self.device, "q4_gemv_lora biases")
         code, xs = _rows(x, in_dim, tokens, self.device, "q4_gemv_lora x")
         ycode, ys = _rows(y, out_dim, tokens, self.device, "q4_gemv_lora y")
         if ycode != code:
