@@ -51,6 +51,8 @@ def _on(t, device: int) -> bool:
 def _rows(t, length: int, count: int, device: int, what: str):
     """(type code, row stride) of a CUDA tensor of `count` rows or more of
     `length` values, each row contiguous."""
+    if not 0 <= count < 2**32:   # the library's count is unsigned, 32 bits
+        raise ValueError(f"{what}: {count} tokens")
     code = _TYPES.get(_type_name(t.dtype))
     if code is None:
         raise ValueError(f"{what}: fp32, bf16 or fp16 rows")
@@ -99,13 +101,17 @@ class Routing:
         values = {"max": _lib.OSM_GROUP_MAX, "top2": _lib.OSM_GROUP_TOP2}
         if score not in scores or group_score not in values:
             raise ValueError("score is softmax or sigmoid, group_score max or top2")
+        top_groups = groups if top_groups is None else top_groups
+        for name, v in (("experts", experts), ("top_k", top_k), ("groups", groups), ("top_groups", top_groups)):
+            if not 0 <= v < 2**32:   # would wrap around in the library's 32 bits
+                raise ValueError(f"routing: {name} is {v}")
         if bias is not None:
             _flat(bias, "torch.float32", experts, bias.device.index, "routing bias")
         self.bias = bias
         self.experts, self.top_k = experts, top_k
         d = self.desc = _lib.RoutingDesc()
         d.experts, d.top_k, d.score = experts, top_k, scores[score]
-        d.groups, d.top_groups = groups, groups if top_groups is None else top_groups
+        d.groups, d.top_groups = groups, top_groups
         d.group_score, d.renormalize, d.scale = values[group_score], int(bool(renormalize)), scale
         d.balance_bias_dev = bias.data_ptr() if bias is not None else None
         self.ref = C.byref(d)
@@ -432,6 +438,8 @@ class Layer:
         """Context.route_scores on this layer's router logits for rows of x
         (fp32); ids and weights are what run_experts takes."""
         dev = self.ctx.device
+        if not 0 <= tokens < 2**32:
+            raise ValueError(f"route_scores x: {tokens} tokens")
         _flat(x, "torch.float32", tokens * self.hidden, dev, "route_scores x")
         routing._check(tokens, ids, weights, mass, dev)
         self.ctx.check(lib().osm_moe_route_scores(self.h, routing.ref, _ptr(x), tokens, _ptr(ids),

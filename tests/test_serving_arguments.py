@@ -107,3 +107,36 @@ def test_q4_tables_that_do_not_hold_the_weights(ctx, library, name, table):
     with pytest.raises(ValueError, match=name):
         project(ctx, projection(**{name: table}))
     assert not library.calls
+
+
+def route(ctx, tokens=None, routing=None, **change):
+    """64 experts, top 8, 4 tokens."""
+    v = dict(logits=OnGpu(torch.zeros(4, 64)), ids=OnGpu(torch.zeros(4, 8, dtype=torch.int32)),
+             weights=OnGpu(torch.zeros(4, 8)), mass=OnGpu(torch.zeros(4)))
+    v.update(change)
+    ctx.route_scores(v["logits"], routing or osm.Routing(64, 8), v["ids"], v["weights"], mass=v["mass"], tokens=tokens)
+
+
+def test_routing_is_called(ctx, library):
+    route(ctx)
+    route(ctx, tokens=3, logits=OnGpu(torch.zeros(4, 70)[:, :64]))
+    assert [(n, a[3:6]) for n, a in library.calls] == [("osm_route_scores", (0, 64, 4)), ("osm_route_scores", (0, 70, 3))]
+
+
+@pytest.mark.parametrize("tokens", [-1, -2**31, -2**32 + 4, 5])
+def test_token_counts(ctx, library, tokens):
+    """Counts that are more than the rows, and negative ones, which the
+    library's unsigned count would take as billions of rows."""
+    with pytest.raises(ValueError, match="rows|token"):
+        route(ctx, tokens=tokens)
+    with pytest.raises(ValueError, match="rows|token"):
+        project(ctx, projection(tokens=tokens))
+    assert not library.calls
+
+
+@pytest.mark.parametrize("field", ["experts", "top_k", "groups", "top_groups"])
+@pytest.mark.parametrize("value", [-1, 2**32 + 1])
+def test_routing_fields_that_would_wrap(field, value):
+    """2**32 + 1 groups are not one group."""
+    with pytest.raises(ValueError, match=field):
+        osm.Routing(**{**dict(experts=64, top_k=8, groups=2, top_groups=1), field: value})
