@@ -140,3 +140,98 @@ def test_routing_fields_that_would_wrap(field, value):
     """2**32 + 1 groups are not one group."""
     with pytest.raises(ValueError, match=field):
         osm.Routing(**{**dict(experts=64, top_k=8, groups=2, top_groups=1), field: value})
+
+
+# ---- each check of test_serving_refusals by its own reason ----
+
+A, B = (3, 8, 128), (3, 32, 8)
+
+
+def table(a_type=torch.bfloat16, b_type=torch.bfloat16, a=None, b=None, **kw):
+    a = torch.zeros(A, dtype=a_type) if a is None else a
+    b = torch.zeros(B, dtype=b_type) if b is None else b
+    return osm.Lora(OnGpu(a), OnGpu(b), **kw)
+
+
+def half(*shape):
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
+def test_adapter_table_is_accepted():
+    t = table(scale=OnGpu(torch.ones(3)), ranks=OnGpu(torch.ones(3, dtype=torch.int32)))
+    assert (t.desc.count, t.desc.rank, t.desc.a_stride, t.desc.b_stride) == (3, 8, 8 * 128, 32 * 8)
+    t = table(a=half(3, 9, 128)[:, :8], b=half(3, 40, 8)[:, :32])   # gaps between adapters
+    assert (t.desc.a_stride, t.desc.b_stride) == (9 * 128, 40 * 8)
+
+
+@pytest.mark.parametrize("reason,kwargs", [
+    ("bf16 or fp16", dict(a_type=torch.float32, b_type=torch.float32)),
+    ("A and B alike", dict(b_type=torch.float16)),
+    (r"B \[n\]\[out\]\[rank\]", dict(b=half(3, 32, 7))), (r"B \[n\]\[out\]\[rank\]", dict(b=half(2, 32, 8))),
+    ("must be contiguous", dict(a=half(3, 128, 8).transpose(1, 2))),
+    ("must be contiguous", dict(b=half(3, 32, 16)[:, :, ::2])),
+    ("must not overlap", dict(a=half(1, 8, 128).expand(A))), ("must not overlap", dict(b=half(1, 32, 8).expand(B))),
+    ("adapter scale", dict(scale=OnGpu(torch.ones(2)))), ("adapter scale", dict(scale=OnGpu(torch.ones(3).double()))),
+    ("adapter scale: not on", dict(scale=OnGpu(torch.ones(3), index=1))),
+    ("adapter ranks", dict(ranks=OnGpu(torch.ones(3)))), ("adapter ranks: not on", dict(ranks=torch.ones(3, dtype=torch.int32)))])
+def test_adapter_table_refused_for(reason, kwargs):
+    with pytest.raises(ValueError, match=reason):
+        table(**kwargs)
+
+
+def test_adapters_of_two_devices_or_none():
+    for a, b in ((half(*A), half(*B)), (OnGpu(half(*A)), OnGpu(half(*B), index=1))):
+        with pytest.raises(ValueError, match="on one GPU"):
+            osm.Lora(a, b)
+
+
+@pytest.mark.parametrize("x,expected", [(torch.zeros(4, 64), (0, 64)), (torch.zeros(4, 70)[:, :64].bfloat16(), (1, 64)),
+                                        (torch.zeros(4, 70, dtype=torch.float16)[:, :64], (2, 70)),
+                                        (torch.zeros(9, 64)[::2], (0, 128))])
+def test_rows_are_accepted(x, expected):
+    assert osm._rows(OnGpu(x), 64, 4, 0, "x") == expected
+
+
+@pytest.mark.parametrize("reason,x", [
+    ("fp32, bf16 or fp16", OnGpu(torch.zeros(4, 64, dtype=torch.int32))),
+    ("4 rows of 64", OnGpu(torch.zeros(4, 60))), ("4 rows of 64", OnGpu(torch.zeros(3, 64))),
+    ("4 rows of 64", OnGpu(torch.zeros(256))), ("must be contiguous", OnGpu(torch.zeros(64, 4).t())),
+    ("must not overlap", OnGpu(torch.zeros(1, 64).expand(4, 64))), ("not on the context's device", torch.zeros(4, 64)),
+    ("not on the context's device", OnGpu(torch.zeros(4, 64), index=1))])
+def test_rows_refused_for(reason, x):
+    with pytest.raises(ValueError, match=reason):
+        osm._rows(x, 64, 4, 0, "x")
+
+
+@pytest.mark.parametrize("reason,change", [
+    ("ids", dict(ids=OnGpu(torch.zeros(4, 7, dtype=torch.int32)))), ("ids", dict(ids=OnGpu(torch.zeros(4, 8, dtype=torch.int64)))),
+    ("weights", dict(weights=OnGpu(torch.zeros(4, 16)[:, ::2]))), ("weights", dict(weights=torch.zeros(4, 8))),
+    ("mass", dict(mass=OnGpu(torch.zeros(3)))), ("logits", dict(logits=OnGpu(torch.zeros(4, 63))))])
+def test_routing_arguments_refused_for(ctx, library, reason, change):
+    with pytest.raises(ValueError, match=f"route.* {reason}"):
+        route(ctx, **change)
+    assert not library.calls
+
+
+@pytest.mark.parametrize("reason,change", [
+    ("of one type", dict(y=OnGpu(torch.zeros(4, 32).bfloat16()))), ("another projection", dict(out_dim=31, y=OnGpu(torch.zeros(4, 31)))),
+    ("indices are missing", dict(adapter=None)), ("adapter", dict(adapter=OnGpu(torch.zeros(4, dtype=torch.int64)))),
+    ("adapter", dict(adapter=OnGpu(torch.zeros(3, dtype=torch.int32)))), ("x: 4 rows", dict(x=OnGpu(torch.zeros(3, 128)))),
+    ("y: 4 rows", dict(y=OnGpu(torch.zeros(4, 33))))])
+def test_projection_arguments_refused_for(ctx, library, reason, change):
+    with pytest.raises(ValueError, match=reason):
+        project(ctx, projection(**change))
+    assert not library.calls
+
+
+def test_routing_choices_and_bias(ctx, library):
+    for kw in (dict(score="tanh"), dict(group_score="mean")):
+        with pytest.raises(ValueError, match="score is softmax or sigmoid"):
+            osm.Routing(64, 8, **kw)
+    for bias in (OnGpu(torch.zeros(63)), OnGpu(torch.zeros(64).half()), torch.zeros(64)):
+        with pytest.raises(ValueError, match="routing bias"):
+            osm.Routing(64, 8, bias=bias)
+    route(ctx, routing=osm.Routing(64, 8, bias=OnGpu(torch.zeros(64))))
+    with pytest.raises(ValueError, match="bias: not on the context's device"):
+        route(ctx, routing=osm.Routing(64, 8, bias=OnGpu(torch.zeros(64), index=1)))
+    assert len(library.calls) == 1
