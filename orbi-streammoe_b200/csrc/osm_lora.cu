@@ -2085,10 +2085,17 @@ cudaError_t launch(const LoraArgs& a, int sms, cudaStream_t s, uint64_t* launche
 constexpr size_t kWsAlign = 1024;
 size_t up(size_t v) { return (v + kWsAlign - 1) / kWsAlign * kWsAlign; }
 
-// Tokens per round of launches: operand planes of at most 256 MB, which keeps
-// the workspace bounded (a multiple of 256 tokens).
+// Tokens per round of launches, a multiple of 256: as many as 256 MB hold the
+// operands, v and lists of, which bounds the workspace beside what W takes (a
+// small K with a large rank has more of v than of x).
 long long block_tokens(const LoraArgs& a) {
-  const long long row = (long long)a.K * (a.x_type == 0 ? 4 : 2);
+  const bool f32 = a.x_type == 0;
+  const int nk = a.K >> 6;
+  long long row = (long long)(nk + bias_chunks(nk, f32)) * 128 * (f32 ? 2 : 1) + 4;   // planes, ex
+  if (a.adapter) {
+    const long long pieces = (a.rank + 15) / 16;
+    row += pieces * 16 * 2 * (f32 ? 3 : 2) + pieces * 8 + 8;                           // v, gran, tok
+  }
   const long long n = (256ll << 20) / row / 256 * 256;
   return n < 256 ? 256 : n;
 }

@@ -68,3 +68,26 @@ def test_parts_that_cancel(torch, ctx, T, K, N, dtype, kind):  # noqa: F811
         tol = tol + 2.0 ** -25
     off = (c.y.double() - y).abs() / tol
     assert float(off.max()) <= 1.0, float(off.max())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_workspace_is_bounded(torch, dtype):  # noqa: F811
+    """Rounds of launches hold the workspace at 256 MB beside what the weights
+    take, also where v (rank 128) is more than x (64 values).  Rows on both sides
+    of a round's end are right."""
+    import osm_b200 as osm
+
+    T, N = 700_001, 8
+    case = Case(torch, T, 64, N, rank=128, n=3, dtype=dtype)
+    ctx = osm.Context(0, max_tokens=4)
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    small = Case(torch, 300, 64, N, rank=128, n=3, dtype=dtype)
+    small.run(ctx)   # what the first call sets up
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    case.run(ctx)
+    torch.cuda.synchronize()
+    assert free - torch.cuda.mem_get_info()[0] <= (256 + 32) << 20
+    y, S, L = case.reference(torch)
+    assert float(((case.y.double() - y).abs() / case.tolerance(torch, y, S, L)).max()) <= 1.0
+    ctx.close()
