@@ -45,7 +45,7 @@ def _type_name(dtype, _names={}):
 
 
 def _on(t, device: int) -> bool:
-    return t.is_cuda and t.get_device() == device
+    return t.get_device() == device   # -1 for a tensor that is on no GPU
 
 
 def _rows(t, length: int, count: int, device: int, what: str):
@@ -77,16 +77,20 @@ def _flat(t, dtype: str, count: int, device: int, what: str):
         raise ValueError(f"{what}: not on the context's device")
 
 
-_Q4_WORDS = frozenset(("torch.int32", "torch.uint32", "torch.uint8"))
-_Q4_SCALES = frozenset(("torch.bfloat16", "torch.uint16", "torch.int16", "torch.uint8"))
+_Q4_WORDS = "torch.int32 torch.uint32 torch.uint8"
+_Q4_SCALES = "torch.bfloat16 torch.uint16 torch.int16 torch.uint8"
 
 
-def _q4_table(t, types, size: int, device: int, what: str):
+def _q4_table(t, types: str, size: int, device: int, what: str, _held={}):
     """A contiguous CUDA tensor of `size` bytes or more in one of `types`."""
-    if _type_name(t.dtype) not in types or t.nbytes < size or not t.is_contiguous():
-        raise ValueError(f"{what}: {size} contiguous bytes in one of {sorted(types)} expected")
+    held = _held.get((t.dtype, types))
+    if held is None:
+        held = _held.setdefault((t.dtype, types), str(t.dtype) in types.split())
+    if held and t.nbytes >= size and t.is_contiguous() and t.get_device() == device:
+        return
     if not _on(t, device):
-        raise ValueError(f"{what}: not on the context's device")
+        raise ValueError(f"q4_gemv_lora {what}: not on the context's device")
+    raise ValueError(f"q4_gemv_lora {what}: {size} contiguous bytes of {types} expected")
 
 
 class Routing:
@@ -255,9 +259,10 @@ class Context:
         (int32, negative: none) of the table `lora`; x and y rows of one type
         (fp32, bf16 or fp16), which may be strided.  W: words (or bytes) of eight
         nibbles, scales and biases in bf16 (or its bits) per group of 64."""
-        _q4_table(packed, _Q4_WORDS, out_dim * in_dim // 2, self.device, "q4_gemv_lora packed")
-        _q4_table(scales_bf16, _Q4_SCALES, out_dim * (in_dim // 64) * 2, self.device, "q4_gemv_lora scales")
-        _q4_table(biases_bf16, _Q4_SCALES, out_dim * (in_dim // 64) * 2, self.device, "q4_gemv_lora biases")
+        size = out_dim * in_dim
+        _q4_table(packed, _Q4_WORDS, size >> 1, self.device, "packed")
+        _q4_table(scales_bf16, _Q4_SCALES, size >> 5, self.device, "scales")
+        _q4_table(biases_bf16, _Q4_SCALES, size >> 5, self.device, "biases")
         code, xs = _rows(x, in_dim, tokens, self.device, "q4_gemv_lora x")
         ycode, ys = _rows(y, out_dim, tokens, self.device, "q4_gemv_lora y")
         if ycode != code:
