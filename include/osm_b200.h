@@ -206,9 +206,11 @@ typedef struct {
  * are neither read nor written, and y must not overlap x.  Sums are held in
  * fp32, y is rounded once; a token's row depends on no other token's row and
  * no other adapter.  A row of x with a NaN or an infinity gives non-finite
- * values in its own y.  The call uses workspace of the context, one block per
- * stream (grown outside stream capture; a captured call carries its own
- * memory in the graph), so calls on two streams do not meet. */
+ * values in its own y.  Workspace is the context's, at most
+ * 256 MB a call beside a fifth of W: the first four streams keep a block each,
+ * calls on others take and return memory in the stream's order, and a captured
+ * call carries its own in the graph, so calls on two streams do not meet and a
+ * stream may be destroyed right behind its calls. */
 int osm_q4_gemv_lora(osm_context* ctx, const uint32_t* packed_dev,
                      const uint16_t* scales_bf16_dev,
                      const uint16_t* biases_bf16_dev, uint32_t out_dim,

@@ -125,15 +125,14 @@ struct osm_context {
                                     // (OSM_DG_DECODE=0: the mma.sync kernels throughout)
   uint32_t dg_min_tokens = 96;      // ... of at least this many tokens (OSM_DG_MIN_TOKENS;
                                     // below it the mma.sync grouped kernels are faster)
-  // workspace of the calls that need no Scratch: one block per stream, so that
-  // calls on two streams do not meet; an outgrown block stays (queued work may
-  // still use it) until the context goes
+  // workspace of the calls that need no Scratch (CallWork): the memory, which
+  // stays until the context goes, and the blocks that the first streams keep of it
+  cudaMemPool_t work_pool = nullptr;
   struct Work {
-    cudaStream_t stream;
-    void* base;
-    size_t bytes;
-  };
-  std::vector<Work> works;
+    unsigned long long stream_id = 0;
+    void* base = nullptr;             // null: free
+    size_t bytes = 0;
+  } works[4];
 };
 
 struct osm_slab {
@@ -378,59 +377,93 @@ int ensure_scratch(osm_context* ctx, size_t T, size_t H, size_t E, size_t k, siz
   return OSM_OK;
 }
 
-// Workspace of one call on the context's stream.  Under stream capture the
-// memory is the graph's own (an allocation and a release node around the
-// call's kernels), so graphs that replay at the same time share nothing;
-// otherwise it is the stream's block.
+// Workspace of one call on the context's stream, such that calls on two streams
+// do not meet.  The first four streams keep a block each, found by the stream's
+// number, which unlike its handle no later stream has again, while an older one's
+// kernels may still run.  Calls on further streams (a program that makes one per
+// request) take their memory before their kernels and give it back behind them,
+// in the stream's order: it passes to another stream only once they have ended.
+// That costs such a call 1 to 4 us.  Under stream capture the memory is the graph's
+// own (an allocation and a release node), so graphs that replay at the same time
+// share nothing.
 struct CallWork {
   osm_context* ctx;
   void* p = nullptr;
-  bool in_graph = false;
+  bool give_back = false;
   explicit CallWork(osm_context* c) : ctx(c) {}
   int get(size_t bytes) {
     if (bytes == 0) return OSM_OK;
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     OSM_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &cap));
     if (cap != cudaStreamCaptureStatusNone) {
-      OSM_CUDA(ctx, cudaMallocAsync(&p, bytes, ctx->stream));
-      in_graph = true;
+      if (int rc = allocated(cudaMallocAsync(&p, bytes, ctx->stream))) return rc;
+      give_back = true;
       return OSM_OK;
     }
-    osm_context::Work* w = nullptr;
-    for (auto& x : ctx->works)
-      if (x.stream == ctx->stream && x.base) w = &x;
-    if (w && w->bytes >= bytes) {
-      p = w->base;
-      return OSM_OK;
-    }
-    // grown by half at least, so that the outgrown blocks stay few and small
-    const size_t want = align_up(std::max(bytes, w ? w->bytes + w->bytes / 2 : bytes), (size_t)1 << 20);
-    void* q = nullptr;
-    if (cudaMalloc(&q, want) != cudaSuccess) {
-      cudaGetLastError();
-      return fail(ctx, OSM_ENOMEM, "workspace allocation failed");
-    }
-    try {
-      if (w) {
-        ctx->retired.push_back(w->base);
-        w->base = q;
-        w->bytes = want;
-      } else {
-        ctx->works.push_back({ctx->stream, q, want});
+    unsigned long long id = 0;
+    OSM_CUDA(ctx, cudaStreamGetId(ctx->stream, &id));
+    osm_context::Work* own = nullptr;
+    for (auto& w : ctx->works) {
+      if (w.base && w.stream_id == id) {
+        own = &w;
+        break;
       }
-    } catch (...) {
-      cudaFree(q);
-      return fail(ctx, OSM_ENOMEM, "workspace bookkeeping failed");
+      if (!w.base && !own) own = &w;
     }
-    p = q;
+    if (own && own->base && own->bytes >= bytes) {
+      p = own->base;
+      return OSM_OK;
+    }
+    if (int rc = pool()) return rc;
+    if (!own) {
+      if (int rc = allocated(cudaMallocFromPoolAsync(&p, bytes, ctx->work_pool, ctx->stream))) return rc;
+      give_back = true;
+      return OSM_OK;
+    }
+    if (own->base) {                  // outgrown, and used by this stream alone
+      OSM_CUDA(ctx, cudaFreeAsync(own->base, ctx->stream));
+      own->base = nullptr;
+    }
+    const size_t want = align_up(bytes, (size_t)1 << 20);
+    if (int rc = allocated(cudaMallocFromPoolAsync(&p, want, ctx->work_pool, ctx->stream))) return rc;
+    *own = {id, p, want};
     return OSM_OK;
   }
   int release(int rc) {
-    if (in_graph) {
+    if (give_back) {
       const cudaError_t e = cudaFreeAsync(p, ctx->stream);
       if (e != cudaSuccess && rc == OSM_OK) return cuda_fail(ctx, e, "workspace release");
     }
     return rc;
+  }
+
+ private:
+  int allocated(cudaError_t e) {
+    if (e == cudaErrorMemoryAllocation) {
+      cudaGetLastError();
+      p = nullptr;
+      return fail(ctx, OSM_ENOMEM, "workspace allocation failed");
+    }
+    return e == cudaSuccess ? OSM_OK : cuda_fail(ctx, e, "workspace");
+  }
+  int pool() {
+    if (ctx->work_pool) return OSM_OK;
+    cudaMemPoolProps props{};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = ctx->device;
+    cudaMemPool_t q = nullptr;
+    OSM_CUDA(ctx, cudaMemPoolCreate(&q, &props));
+    uint64_t keep = UINT64_MAX;   // not given back to the device at every synchronisation
+    int no = 0;                   // no stream is made to wait for another one's memory
+    cudaError_t e = cudaMemPoolSetAttribute(q, cudaMemPoolAttrReleaseThreshold, &keep);
+    if (e == cudaSuccess) e = cudaMemPoolSetAttribute(q, cudaMemPoolReuseAllowInternalDependencies, &no);
+    if (e != cudaSuccess) {
+      cudaMemPoolDestroy(q);
+      return cuda_fail(ctx, e, "workspace pool");
+    }
+    ctx->work_pool = q;
+    return OSM_OK;
   }
 };
 
@@ -1112,7 +1145,9 @@ int osm_context_destroy(osm_context* ctx) {
   cudaStreamSynchronize(ctx->stream);
   if (ctx->sc.base) cudaFree(ctx->sc.base);
   for (void* p : ctx->retired) cudaFree(p);
-  for (const auto& w : ctx->works) cudaFree(w.base);
+  for (const auto& w : ctx->works)
+    if (w.base) cudaFree(w.base);
+  if (ctx->work_pool) cudaMemPoolDestroy(ctx->work_pool);
   if (ctx->status_blk) cudaFree(ctx->status_blk);
   for (const ProfRec& r : ctx->recs) {
     cudaEventDestroy(r.a);

@@ -2158,7 +2158,7 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
       off += up((size_t)a.l_blocks * 4);
     }
     a.v = reinterpret_cast<float*>(base + off);
-    off += up((size_t)a.tokens * a.v_stride * (dec ? 4 : 2 * a.v_planes));
+    if (!a.v_self) off += up((size_t)a.tokens * a.v_stride * (dec ? 4 : 2 * a.v_planes));
   }
   return off;
 }

@@ -91,3 +91,47 @@ def test_workspace_is_bounded(torch, dtype):  # noqa: F811
     y, S, L = case.reference(torch)
     assert float(((case.y.double() - y).abs() / case.tolerance(torch, y, S, L)).max()) <= 1.0
     ctx.close()
+
+
+def test_streams_that_come_and_go(torch):  # noqa: F811
+    """Streams destroyed right behind their calls, whose handles the next ones may
+    have again: each call has its own workspace while it runs, and what the calls
+    of 60 streams take is not more than those in flight need."""
+    import ctypes
+
+    import osm_b200 as osm
+
+    rt = torch.cuda.cudart()
+    ctx = osm.Context(0, max_tokens=4)
+    cases = [Case(torch, T, K, 512, n=n, rank=r, dtype=d, seed=i) for i, (T, K, n, r, d) in
+             enumerate([(1500, 1024, 9, 24, "fp32"), (90, 512, 40, 16, "bf16"), (700, 2048, 5, 64, "fp16"),
+                        (3, 4096, 3, 100, "fp32")])]
+    want = []
+    ctx.set_stream(0)
+    for c in cases:
+        want.append(c.run(ctx).clone())
+    torch.cuda.synchronize()
+
+    def generation():
+        for c in cases:
+            c.yw.fill_(-7)
+        torch.cuda.synchronize()
+        for c in cases:
+            s = ctypes.c_void_p()
+            assert int(rt.cudaStreamCreate(ctypes.addressof(s))) == 0
+            ctx.set_stream(s.value)
+            for _ in range(3):
+                c.run(ctx)
+            assert int(rt.cudaStreamDestroy(s.value)) == 0
+        torch.cuda.synchronize()
+        for c, w in zip(cases, want):
+            assert torch.equal(c.y, w)
+
+    for _ in range(5):
+        generation()
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(10):
+        generation()
+    assert free - torch.cuda.mem_get_info()[0] <= 64 << 20
+    ctx.set_stream(0)
+    ctx.close()
