@@ -12,6 +12,36 @@ from test_gpu_lora import Case, ctx, torch  # noqa: F401  (fixtures)
 pytestmark = pytest.mark.gpu
 
 
+def tolerance(torch, c, y, S, L):  # noqa: F811
+    """That of test_gpu_lora without its term 2^-11 C for 16-bit rows.
+
+    Per group: c = bias + 8 scale is hi + lo of fp16, within 2^-24 of itself; the
+    sum of x is taken in fp32 (10 half-ulps, 2^-24 each, of the sum of magnitudes)
+    and held as hi + lo, 2^-24; the product of the two lo parts is left out, 2^-24:
+    under 16 2^-23 C together.  Steps of 16: K / 16 of the products, 3 K / 1024 of
+    the biases' columns, rounded up to a stage of 4: under K / 8 + K / 256 + 4, each
+    with a loss of 2^-23 of the sum of magnitudes at most.  v is held in 16 bits for
+    16-bit rows, 2^-15 L as there; y of fp16 is rounded to a multiple of 2^-24 at
+    the least."""
+    S = S[0]
+    tol = (torch.finfo(c.dt).eps / 2 * y.abs() + (c.K / 8 + c.K / 256 + 20) * 2.0 ** -23 * (S + L)
+           + c.rank * 2.0 ** -23 * L + 1e-30)
+    if c.dt != torch.float32:
+        tol = tol + 2.0 ** -15 * L
+    if c.dt == torch.float16:
+        tol = tol + 2.0 ** -25
+    return tol
+
+
+def check(torch, ctx, c, lora=True):  # noqa: F811
+    c.run(ctx, lora)
+    torch.cuda.synchronize()
+    y, S, L = c.reference(torch, lora)
+    off = (c.y.double() - y).abs() / tolerance(torch, c, y, S, L)
+    assert float(off.max()) <= 1.0, float(off.max())  # NaN fails too
+    assert (c.yw[c.T:] == -7).all() and (c.yw[:, c.N:] == -7).all()
+
+
 # Tiles of 96 to 128 fp32 tokens take the three planes of v in two passes, and
 # fp16 adapters their low part in further ones; a CTA's share of K is 17, 17, 13
 # and 9 stages here, so that the last of these passes would open a partial sum.
@@ -45,29 +75,9 @@ def one_sided(torch, T, K, N, dtype, kind, seed=0):
 @pytest.mark.parametrize("T,K,N", [(3, 512, 96), (40, 512, 96), (300, 512, 96), (300, 1408, 2048), (1100, 64, 200),
                                    (4200, 2048, 130)])
 def test_parts_that_cancel(torch, ctx, T, K, N, dtype, kind):  # noqa: F811
-    """No operand of the two parts has fewer than 22 bits, whatever the rows'
-    type: the tolerance of test_gpu_lora without its term 2^-11 C.
-
-    Per group: c = bias + 8 scale is hi + lo of fp16, within 2^-24 of itself; the
-    sum of x is taken in fp32 (10 half-ulps, 2^-24 each, of the sum of magnitudes)
-    and held as hi + lo, 2^-24; the product of the two lo parts is left out, 2^-24:
-    under 16 2^-23 C together.  Steps of 16: K / 16 of the products, 3 K / 1024 of
-    the biases' columns, rounded up to a stage of 4: under K / 8 + K / 256 + 4, each
-    with a loss of 2^-23 of the sum of magnitudes at most.  v is held in 16 bits for
-    16-bit rows, 2^-15 L as there; y of fp16 is rounded to a multiple of 2^-24 at
-    the least."""
+    """No operand of the two parts has fewer than 22 bits, whatever the rows' type."""
     c = one_sided(torch, T, K, N, dtype, kind, seed=K)
-    c.run(ctx)
-    torch.cuda.synchronize()
-    y, (S, C), L = c.reference(torch)
-    tol = (torch.finfo(c.dt).eps / 2 * y.abs() + (K / 8 + K / 256 + 20) * 2.0 ** -23 * (S + L) + c.rank * 2.0 ** -23 * L
-           + 1e-30)
-    if dtype != "fp32":
-        tol = tol + 2.0 ** -15 * L
-    if dtype == "fp16":
-        tol = tol + 2.0 ** -25
-    off = (c.y.double() - y).abs() / tol
-    assert float(off.max()) <= 1.0, float(off.max())
+    check(torch, ctx, c)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
@@ -88,8 +98,7 @@ def test_workspace_is_bounded(torch, dtype):  # noqa: F811
     case.run(ctx)
     torch.cuda.synchronize()
     assert free - torch.cuda.mem_get_info()[0] <= (256 + 32) << 20
-    y, S, L = case.reference(torch)
-    assert float(((case.y.double() - y).abs() / case.tolerance(torch, y, S, L)).max()) <= 1.0
+    check(torch, ctx, case)
     ctx.close()
 
 
@@ -135,3 +144,213 @@ def test_streams_that_come_and_go(torch):  # noqa: F811
     assert free - torch.cuda.mem_get_info()[0] <= 64 << 20
     ctx.set_stream(0)
     ctx.close()
+
+
+# Shares of K of 1 to 16 stages in all remainders of 4 (a partial sum of fp32
+# rows), on 1, 2, 4 and 8 CTAs a tile, tiles of 16 to 240 tokens whose last one
+# holds 12 to 172; below and above 4096 tokens, where another kernel computes v.
+SIZES = [(300, 64, 72, 7, 3), (300, 192, 72, 33, 3), (300, 256, 136, 128, 4), (300, 832, 300, 65, 5),
+         (300, 2048, 72, 1, 3), (1100, 320, 200, 33, 6), (1100, 1088, 640, 7, 4), (1100, 2112, 72, 128, 3),
+         (1100, 128, 1500, 65, 9), (4200, 192, 136, 128, 6), (4200, 448, 72, 7, 40), (4200, 64, 130, 65, 3),
+         (4200, 704, 1024, 33, 5), (700, 896, 2048, 16, 3), (2500, 704, 1500, 24, 7)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("half", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,K,N,rank,n", SIZES)
+def test_ranks_and_types(torch, ctx, T, K, N, rank, n, half, dtype):  # noqa: F811
+    """Every type of row beside every type of adapter, ranks that end inside a
+    piece of 16 and inside the pieces of one pass over A, adapters of rank 0."""
+    ctx.status()
+    check(torch, ctx, Case(torch, T, K, N, rank=rank, n=n, dtype=dtype, half=half, ranks=rank > 1, seed=rank))
+    assert ctx.status()[0] == 0
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("T,K,N", [(300, 512, 200), (1100, 192, 130), (4200, 448, 136)])
+def test_without_adapters(torch, ctx, T, K, N, dtype):  # noqa: F811
+    check(torch, ctx, Case(torch, T, K, N, dtype=dtype), lora=False)
+    c = Case(torch, T, K, N, dtype=dtype)
+    c.adapter.fill_(-1)  # a table, but no token uses it
+    check(torch, ctx, c)
+
+
+@pytest.mark.parametrize("what", ["tables", "adapters", "x"])
+@pytest.mark.parametrize("dtype,half", [("fp32", "bf16"), ("fp32", "fp16"), ("bf16", "bf16"), ("bf16", "fp16"),
+                                        ("fp16", "fp16")])
+@pytest.mark.parametrize("T", [300, 1100, 4200])
+def test_unaligned(torch, ctx, T, dtype, half, what):  # noqa: F811
+    """One element (one word) past a 16-byte boundary: W's tables and the lists, A
+    and B with gaps between adapters, or the rows of x, with NaN in the gaps."""
+    c = Case(torch, T, 320, 136, rank=21, n=5, dtype=dtype, half=half, ranks=True)
+    if what == "tables":
+        for name in ("packed", "scales", "biases", "gain", "ranks", "adapter"):
+            v = getattr(c, name)
+            buf = torch.empty(v.numel() + 1, dtype=v.dtype, device="cuda")
+            buf[1:] = v.reshape(-1)
+            setattr(c, name, buf[1:].view(v.shape))
+    elif what == "adapters":
+        for name in ("a", "b"):
+            v = getattr(c, name)
+            m = v[0].numel()
+            buf = torch.full((1 + c.n * (m + 3),), float("nan"), dtype=v.dtype, device="cuda")
+            w = buf[1:].as_strided(v.shape, (m + 3, v.shape[2], 1))
+            w.copy_(v)
+            setattr(c, name, w)
+    else:
+        buf = torch.full((1 + T * 323,), float("nan"), dtype=c.dt, device="cuda")
+        x = buf[1:].as_strided((T, 320), (323, 1))
+        x.copy_(c.x)
+        c.x = x
+    check(torch, ctx, c)
+
+
+@pytest.mark.parametrize("xpad,ypad", [(1, 1), (8, 8), (0, 1), (3, 0)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("T", [300, 4200])
+def test_strides(torch, ctx, T, dtype, xpad, ypad):  # noqa: F811
+    check(torch, ctx, Case(torch, T, 320, 136, dtype=dtype, xpad=xpad, ypad=ypad))
+
+
+@pytest.mark.parametrize("half", ["bf16", "fp16"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("T", [1100, 4200])
+def test_rows_and_adapters_do_not_meet(torch, ctx, T, dtype, half):  # noqa: F811
+    """Non-finite values in one adapter or one token's row stay there."""
+    c = Case(torch, T, 256, 160, n=4, rank=20, dtype=dtype, half=half)
+    c.adapter = (torch.arange(T, device="cuda") % 4).int()
+    c.run(ctx)
+    good = c.y.clone()
+    c.a[2, 17, 5] = float("nan")
+    c.b[1, 7, 2] = float("inf")
+    c.b[1, 9, 19] = float("nan")
+    c.x[0, 1] = float("nan")
+    c.x[T - 1, 9] = float("inf")
+    c.run(ctx)
+    torch.cuda.synchronize()
+    ad = c.adapter
+    clean = (ad != 2) & (ad != 1)
+    clean[0] = clean[T - 1] = False
+    assert torch.equal(c.y[clean], good[clean])
+    one = ad == 1
+    one[T - 1] = False
+    cols = torch.ones(160, dtype=torch.bool, device="cuda")
+    cols[7] = cols[9] = False
+    assert torch.equal(c.y[one][:, cols], good[one][:, cols])
+    assert not torch.isfinite(c.y[one][:, ~cols].float()).any()
+    assert torch.isnan(c.y[(ad == 2)]).all()
+    assert not torch.isfinite(c.y[0].float()).any() and not torch.isfinite(c.y[T - 1].float()).any()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("T", [300, 4200])
+def test_rows_behind_an_adapters_rank_are_not_used(torch, ctx, T, dtype):  # noqa: F811
+    c = Case(torch, T, 128, 96, rank=72, n=4, ranks=True, dtype=dtype)
+    c.ranks.copy_(torch.tensor([0, 9, 72, 33]))
+    c.a[0] = c.b[0] = float("nan")
+    c.a[1, 9:], c.a[3, 33:] = float("nan"), float("inf")
+    c.b[1, :, 9:], c.b[3, :, 33:] = float("inf"), float("nan")
+    check(torch, ctx, c)
+
+
+@pytest.mark.parametrize("T", [300, 4200])
+def test_index_past_the_table(torch, ctx, T):  # noqa: F811
+    c = Case(torch, T, 128, 64, n=2)
+    c.adapter[1] = -2**31
+    ctx.status()
+    check(torch, ctx, c)
+    assert ctx.status()[0] == 0
+    c.adapter[0] = 2
+    c.adapter[T - 1] = 2**31 - 1
+    check(torch, ctx, c)  # the reference takes neither as an adapter
+    assert ctx.status()[0] == 256
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("T", [300, 1100, 4200])
+def test_scales_of_every_size(torch, ctx, T, dtype):  # noqa: F811
+    """Rows of x and of W from 1e-27 to 1e+27, zero rows among them."""
+    c = Case(torch, T, 256, 64, dtype=dtype)
+    row = torch.logspace(-15, 15, 64, device="cuda")[:, None]
+    c.scales, c.biases = (c.scales.float() * row).bfloat16(), (c.biases.float() * row).bfloat16()
+    c.b = (c.b.float() * row).to(c.b.dtype)
+    c.x.mul_(torch.logspace(-12, 12, T, device="cuda")[:, None].to(c.dt))
+    c.x[:, ::7] *= 1e-4
+    c.x[::5] = 0
+    check(torch, ctx, c)
+    assert (c.y[::5] == 0).all()
+
+
+@pytest.mark.parametrize("T", [300, 1100])
+def test_sublayer_of_many_requests(torch, T):  # noqa: F811
+    """A sublayer as a server of many requests runs it: a grouped sigmoid router
+    with a balance bias in front of the layer's routed experts, and beside them a
+    dense branch of three Q4 projections with an adapter per request (gate, up,
+    SwiGLU, down), whose output is the experts' residual; everything captured into
+    one graph and replayed with other inputs."""
+    import osm_b200 as osm
+    from gpu_util import MoeFixture
+
+    H, E, I, k = 512, 32, 256, 4
+    f = MoeFixture(torch, H, E, I, k, seed=31, max_tokens=T)
+    gate, up = (Case(torch, T, H, I, n=6, seed=s, dtype="fp32", half="fp16") for s in (1, 2))
+    down = Case(torch, T, I, H, n=6, seed=3, dtype="fp32", half="fp16")
+    up.x, up.adapter, down.adapter = gate.x, gate.adapter, gate.adapter
+    bias = 0.05 * torch.randn(E, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    r = osm.Routing(E, k, score="sigmoid", bias=bias, groups=4, top_groups=2, group_score="top2", scale=1.5)
+    ids = torch.zeros(T, k, dtype=torch.int32, device="cuda")
+    w = torch.zeros(T, k, device="cuda")
+    x, h = gate.x, torch.empty(T, I, device="cuda")
+    dense, out, logits = (torch.empty(T, n, device="cuda") for n in (H, H, E))
+    down.x, down.y = h, dense
+
+    def step():
+        f.layer.route_scores(x, T, r, ids, w)
+        g, u = gate.run(f.ctx), up.run(f.ctx)
+        f.ctx.swiglu(g, u, h)
+        down.run(f.ctx)
+        f.layer.run_experts(x, T, ids, w, out, residual=dense)
+
+    def verify():
+        torch.cuda.synchronize()
+        assert f.ctx.status()[0] == 0
+        gy, uy = gate.reference(torch)[0], up.reference(torch)[0]
+        down.x = gy / (1 + torch.exp(-gy)) * uy
+        dy = down.reference(torch)[0]
+        down.x = h
+        f.layer.route_qwen_top_k_logits(x, T, logits)
+        torch.cuda.synchronize()
+        s = torch.sigmoid(logits.double())
+        c = (s + bias.double()).view(T, 4, E // 4)
+        value = c.sort(2, descending=True).values[:, :, :2].sum(2)
+        kept = torch.zeros(T, 4, dtype=torch.bool, device="cuda").scatter_(1, value.topk(2, 1).indices, True)
+        pick = c.masked_fill(~kept[:, :, None], -9).view(T, E).topk(k, 1).indices
+        assert torch.equal(ids.long(), pick)
+        sw = s.gather(1, pick)
+        sw = 1.5 * sw / sw.sum(1, keepdim=True)
+        assert torch.allclose(w.double(), sw, rtol=1e-5)
+        mats = {e: [torch.from_numpy(m).double().cuda() for m in v] for e, v in f.experts(range(E)).items()}
+
+        def run(m):
+            gx = x.double() @ m[0].T
+            return (gx / (1 + torch.exp(-gx)) * (x.double() @ m[1].T)) @ m[2].T
+
+        shared = run([torch.from_numpy(m).double().cuda() for m in f.shared_f32()])
+        ref = dy + torch.sigmoid(x.double() @ torch.from_numpy(f.sg).double().cuda())[:, None] * shared
+        for e in range(E):
+            ref += run(mats[e]) * (sw * (pick == e)).sum(1, keepdim=True)
+        off = (out.double() - ref).abs().amax(1) / ref.abs().amax(1)
+        assert float(off.max()) <= 1e-4, float(off.max())
+
+    step()
+    verify()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        f.ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+        step()
+    f.ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    x.copy_(torch.randn(T, H, device="cuda", generator=torch.Generator("cuda").manual_seed(T)))
+    gate.adapter.copy_(gate.adapter.flip(0))
+    out.fill_(-7)
+    graph.replay()
+    verify()
