@@ -1100,7 +1100,6 @@ int osm_context_create(int device, uint32_t max_tokens, osm_context** out) {
   osm::init_prefill_attributes(ctx->max_smem);
   osm::init_tc_attributes(ctx->max_smem);
   osm::init_dg_attributes(ctx->max_smem);
-  osm::init_lora_attributes(ctx->max_smem);
   {
     const char* v = std::getenv("OSM_DISABLE_TC");
     ctx->tc_enabled = !(v && v[0] && v[0] != '0');

@@ -496,7 +496,6 @@ struct LoraArgs {
   int v_blocks, v_slots, l_blocks, w_blocks, row_threads, after_v, v_self;
   int x_vec, w_vec, m_vec, a_vec, b_vec;  // 16-byte aligned rows (m: scales and biases)
 };
-cudaError_t init_lora_attributes(int max_smem);
 size_t lora_workspace(const LoraArgs& a, int sms);
 cudaError_t launch_lora(const LoraArgs& a, void* workspace, int sms, cudaStream_t s, uint64_t* launches);
 

@@ -48,6 +48,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "osm_common.cuh"
@@ -1994,9 +1995,24 @@ void lg_shape(const LoraArgs& a, int sms, int* NT, int* split) {
   }
 }
 
-template <typename K>
-cudaError_t launch_cfg(K kernel, unsigned grid, unsigned block, size_t smem, int cluster, cudaStream_t s,
+// `most`: dynamic shared memory of any launch of the kernel.  More than 48 KB
+// with the static part (under 8 KB here) is asked for at the first launch on a
+// device that needs it, not when a context is made: that loads the kernel, and
+// all of this file's take 24 ms.
+template <auto KERNEL>
+cudaError_t launch_cfg(unsigned grid, unsigned block, size_t smem, size_t most, int cluster, cudaStream_t s,
                        const LoraArgs& a) {
+  if (smem > (40 << 10)) {
+    static std::atomic<uint64_t> asked{0};   // a bit per device
+    int device = 0;
+    if (const cudaError_t e = cudaGetDevice(&device)) return e;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (!(asked.load(std::memory_order_relaxed) & bit)) {
+      const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+      if (e != cudaSuccess) return e;
+      asked.fetch_or(bit, std::memory_order_relaxed);
+    }
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
@@ -2014,15 +2030,15 @@ cudaError_t launch_cfg(K kernel, unsigned grid, unsigned block, size_t smem, int
     cfg.numAttrs = 2;
   }
   cfg.attrs = attr;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  return cudaLaunchKernelEx(&cfg, KERNEL, a);
 }
 
 template <int XT, int AT, int TT>
 cudaError_t launch_decode(const LoraArgs& a, cudaStream_t s) {
   const size_t sm = (size_t)a.tokens * a.K * 4;
   if (TT >= 4 && dec_rows(a) == 2)
-    return launch_cfg(lora_decode_kernel<XT, AT, TT, 2>, dec_blocks(a), kDecWarps * 32, sm, 1, s, a);
-  return launch_cfg(lora_decode_kernel<XT, AT, TT, 1>, dec_blocks(a), kDecWarps * 32, sm, 1, s, a);
+    return launch_cfg<lora_decode_kernel<XT, AT, TT, 2>>(dec_blocks(a), kDecWarps * 32, sm, kDecSmem, 1, s, a);
+  return launch_cfg<lora_decode_kernel<XT, AT, TT, 1>>(dec_blocks(a), kDecWarps * 32, sm, kDecSmem, 1, s, a);
 }
 
 // The most rows per CTA that still give every SM one (for 16-bit rows 64 rows
@@ -2033,12 +2049,16 @@ cudaError_t launch_batch(const LoraArgs& a, int sms, cudaStream_t s) {
   const unsigned tt = (unsigned)((a.tokens + 8 * NT - 1) / (8 * NT));
   const size_t v = a.adapter ? (size_t)8 * NT * a.v_stride * 4 : 0;
   auto tiles = [&](int mt) { return (unsigned)((a.N + 16 * mt - 1) / (16 * mt)) * tt; };
+  auto go = [&](auto mt) {
+    constexpr int MT = decltype(mt)::value;
+    constexpr size_t bytes = BatSmem<XT, MT, NT>::BYTES;
+    return launch_cfg<lora_batch_kernel<XT, AT, MT, NT>>(tiles(MT), kBatWarps * 32, bytes + v,
+                                                         bytes + 8 * NT * kBatRank * 4, 1, s, a);
+  };
   if constexpr (XT == 0)
-    if (tiles(4) >= (unsigned)sms)
-      return launch_cfg(lora_batch_kernel<XT, AT, 4, NT>, tiles(4), kBatWarps * 32, BatSmem<XT, 4, NT>::BYTES + v, 1, s, a);
-  if (tiles(2) >= (unsigned)sms)
-    return launch_cfg(lora_batch_kernel<XT, AT, 2, NT>, tiles(2), kBatWarps * 32, BatSmem<XT, 2, NT>::BYTES + v, 1, s, a);
-  return launch_cfg(lora_batch_kernel<XT, AT, 1, NT>, tiles(1), kBatWarps * 32, BatSmem<XT, 1, NT>::BYTES + v, 1, s, a);
+    if (tiles(4) >= (unsigned)sms) return go(std::integral_constant<int, 4>{});
+  if (tiles(2) >= (unsigned)sms) return go(std::integral_constant<int, 2>{});
+  return go(std::integral_constant<int, 1>{});
 }
 
 template <int XT, int AT>
@@ -2050,8 +2070,8 @@ cudaError_t launch(const LoraArgs& a, int sms, cudaStream_t s, uint64_t* launche
     };
     const cudaError_t e =
         a.tokens * a.rank <= 1024
-            ? launch_cfg(lora_v_rows_kernel<XT, AT, 1>, blocks(1), kRowWarps * 32, 0, 1, s, a)
-            : launch_cfg(lora_v_rows_kernel<XT, AT, 4>, blocks(4), kRowWarps * 32, 0, 1, s, a);
+            ? launch_cfg<lora_v_rows_kernel<XT, AT, 1>>(blocks(1), kRowWarps * 32, 0, 0, 1, s, a)
+            : launch_cfg<lora_v_rows_kernel<XT, AT, 4>>(blocks(4), kRowWarps * 32, 0, 0, 1, s, a);
     if (e != cudaSuccess) return e;
     if (launches) *launches += 1;
   }
@@ -2059,14 +2079,14 @@ cudaError_t launch(const LoraArgs& a, int sms, cudaStream_t s, uint64_t* launche
   const long long row_blocks = dec ? 0 : a.row_threads == 32 ? rows / kPrepWarps : rows;
   const long long prep = a.v_blocks + a.l_blocks + a.w_blocks + row_blocks;
   if (a.after_v) {
-    const cudaError_t e = launch_cfg(lora_v_kernel<XT, AT>, (unsigned)a.after_v * VBig<XT>::KSPLIT, VBig<XT>::THREADS,
-                                     VBig<XT>::BYTES, VBig<XT>::KSPLIT, s, a);
+    const cudaError_t e = launch_cfg<lora_v_kernel<XT, AT>>((unsigned)a.after_v * VBig<XT>::KSPLIT, VBig<XT>::THREADS,
+                                                            VBig<XT>::BYTES, VBig<XT>::BYTES, VBig<XT>::KSPLIT, s, a);
     if (e != cudaSuccess) return e;
     if (launches) *launches += 1;
   }
   if (prep) {
-    const cudaError_t e = launch_cfg(lora_prep_kernel<XT, AT>, (unsigned)prep, kPrepThreads, a.v_blocks ? kPrepRed : 0, 1,
-                                     s, a);
+    const cudaError_t e = launch_cfg<lora_prep_kernel<XT, AT>>((unsigned)prep, kPrepThreads, a.v_blocks ? kPrepRed : 0,
+                                                               kPrepRed, 1, s, a);
     if (e != cudaSuccess) return e;
     if (launches) *launches += 1;
   }
@@ -2079,7 +2099,7 @@ cudaError_t launch(const LoraArgs& a, int sms, cudaStream_t s, uint64_t* launche
   }
   const long long tiles = (long long)((a.N + kLgM - 1) / kLgM) * ((a.tokens + a.NT - 1) / a.NT);
   const unsigned grid = (unsigned)(a.split > 1 ? tiles * a.split : tiles < sms ? tiles : sms);
-  return launch_cfg(lora_gemm_kernel<XT, AT>, grid, kLgThreads, kLgSmem, a.split, s, a);
+  return launch_cfg<lora_gemm_kernel<XT, AT>>(grid, kLgThreads, kLgSmem, kLgSmem, a.split, s, a);
 }
 
 constexpr size_t kWsAlign = 1024;
@@ -2163,39 +2183,7 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
   return off;
 }
 
-template <int XT, int AT>
-cudaError_t set_smem() {
-  cudaError_t e = cudaFuncSetAttribute(lora_v_kernel<XT, AT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)VBig<XT>::BYTES);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(lora_gemm_kernel<XT, AT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLgSmem);
-  auto dec = [&](auto kernel) {
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kDecSmem);
-  };
-  dec(lora_decode_kernel<XT, AT, 1, 1>);
-  dec(lora_decode_kernel<XT, AT, 2, 1>);
-  dec(lora_decode_kernel<XT, AT, 4, 1>);
-  dec(lora_decode_kernel<XT, AT, 4, 2>);
-  constexpr int NT = XT == 0 ? 2 : 4;
-  auto bat = [&](auto kernel, size_t bytes) {
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(bytes + 8 * NT * kBatRank * 4));
-  };
-  bat(lora_batch_kernel<XT, AT, 1, NT>, BatSmem<XT, 1, NT>::BYTES);
-  bat(lora_batch_kernel<XT, AT, 2, NT>, BatSmem<XT, 2, NT>::BYTES);
-  if constexpr (XT == 0) bat(lora_batch_kernel<XT, AT, 4, NT>, BatSmem<XT, 4, NT>::BYTES);
-  return e;
-}
-
 }  // namespace
-
-cudaError_t init_lora_attributes(int max_smem) {
-  if ((int)kLgSmem > max_smem) return cudaErrorInvalidConfiguration;
-  cudaError_t e = set_smem<0, 1>();
-  if (e == cudaSuccess) e = set_smem<0, 2>();
-  if (e == cudaSuccess) e = set_smem<1, 1>();
-  if (e == cudaSuccess) e = set_smem<1, 2>();
-  if (e == cudaSuccess) e = set_smem<2, 1>();
-  if (e == cudaSuccess) e = set_smem<2, 2>();
-  return e;
-}
 
 size_t lora_workspace(const LoraArgs& args, int sms) {
   const long long most = block_tokens(args);
