@@ -1046,7 +1046,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) lora_v_rows_kernel(const __gri
 // their order, then B_a v in fp32; v comes from the kernel before, which this one
 // waits for only there.
 constexpr int kBatWarps = 8;
-constexpr int kBatRank = 128;   // v in shared memory, most
+constexpr int kBatRank = 128;   // the largest rank of any call: v in shared memory
 
 template <int XT, int MT, int NT>
 struct BatSmem {
@@ -1505,7 +1505,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
             if (F32 && (k_lo + c < nk || ((k_lo + c - nk) & 1) == 0)) issue((uint32_t)C::NMAX * 128, idf);
           } else {
             const int pass = (c - nkm) % passes;
-            const bool lo_part = pass >= hi;
+            const bool lo_part = BLO && pass >= hi;
             const int p0 = (lo_part ? pass - hi : pass) * vpl;
             const int planes = min(lo_part ? C::NV - 1 : C::NV, p0 + vpl) - p0;
             for (int p = 0; p < planes; ++p) issue((uint32_t)(p * npad * 128), idb);
@@ -1663,7 +1663,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
         const uint32_t oc = os + (uint32_t)c;
         const int st = (int)(oc % kLgRO);
         const int blk = block_of(c), pass = (c - nkm) % passes;
-        const bool lo_part = pass >= hi;
+        const bool lo_part = BLO && pass >= hi;
         const int p0 = (lo_part ? pass - hi : pass) * vpl;
         const int planes = min(lo_part ? C::NV - 1 : C::NV, p0 + vpl) - p0;
         const bool here = c == c_first;
@@ -1952,7 +1952,7 @@ bool v_by_self(const LoraArgs& a) {
 constexpr int kBatTokens = 256;
 constexpr double kBatWork = 1e9;
 bool batches(const LoraArgs& a) {
-  return !decodes(a) && a.tokens <= kBatTokens && (!a.adapter || a.rank <= kBatRank) &&
+  return !decodes(a) && a.tokens <= kBatTokens &&
          (double)a.tokens * a.N * a.K * (a.x_type == 0 ? 3 : 1) <= kBatWork;
 }
 bool v_by_rows(const LoraArgs& a) { return (decodes(a) || batches(a)) && !v_by_self(a); }
@@ -2002,14 +2002,17 @@ void lg_shape(const LoraArgs& a, int sms, int* NT, int* split) {
 template <auto KERNEL>
 cudaError_t launch_cfg(unsigned grid, unsigned block, size_t smem, size_t most, int cluster, cudaStream_t s,
                        const LoraArgs& a) {
-  if (smem > (40 << 10)) {
-    static std::atomic<uint64_t> asked{0};   // a bit per device
+  static std::atomic<uint64_t> asked{0};   // a bit per device
+  auto ask = [&]() {
+    return cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+  };
+  const bool big = smem > (40 << 10);
+  if (big) {
     int device = 0;
     if (const cudaError_t e = cudaGetDevice(&device)) return e;
     const uint64_t bit = device < 64 ? 1ull << device : 0;
     if (!(asked.load(std::memory_order_relaxed) & bit)) {
-      const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
-      if (e != cudaSuccess) return e;
+      if (const cudaError_t e = ask()) return e;
       asked.fetch_or(bit, std::memory_order_relaxed);
     }
   }
@@ -2030,7 +2033,12 @@ cudaError_t launch_cfg(unsigned grid, unsigned block, size_t smem, size_t most, 
     cfg.numAttrs = 2;
   }
   cfg.attrs = attr;
-  return cudaLaunchKernelEx(&cfg, KERNEL, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, KERNEL, a);
+  if (e == cudaErrorInvalidValue && big && ask() == cudaSuccess) {   // a device reset since then has undone it
+    cudaGetLastError();
+    e = cudaLaunchKernelEx(&cfg, KERNEL, a);
+  }
+  return e;
 }
 
 template <int XT, int AT, int TT>
