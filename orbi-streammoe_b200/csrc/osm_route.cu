@@ -458,7 +458,10 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_scores_kernel(const __
   float s = 0.0f;
   if (lane < a.k) s = a.sigmoid ? 1.0f / (1.0f + expf(-lg)) : expf(lg - m) / sum;
   const float mass = warp_sum(s);
-  if (!(mass > 1e-30f)) {
+  // a score that fp32 does not hold (a bias can pick it): of no weight beside a
+  // large mass, but a small one brings it back into range
+  const bool under = a.renorm && __any_sync(kAll, lane < a.k && s < 1e-36f);
+  if (!(mass > 1e-30f) || (under && mass < 0.1f)) {
     route_scores_64<TYPE>(a, t, c64);
     return;
   }
