@@ -44,10 +44,6 @@ def _type_name(dtype, _names={}):
     return name
 
 
-def _on(t, device: int) -> bool:
-    return t.get_device() == device   # -1 for a tensor that is on no GPU
-
-
 def _rows(t, length: int, count: int, device: int, what: str):
     """(type code, row stride) of a CUDA tensor of `count` rows or more of
     `length` values, each row contiguous."""
@@ -62,7 +58,7 @@ def _rows(t, length: int, count: int, device: int, what: str):
     step, inner = t.stride()
     if (length > 1 and inner != 1) or (count > 1 and step < length):
         raise ValueError(f"{what}: rows must be contiguous and must not overlap")
-    if not _on(t, device):
+    if t.get_device() != device:   # -1 for a tensor that is on no GPU
         raise ValueError(f"{what}: not on the context's device")
     return code, step if count > 1 else 0
 
@@ -73,24 +69,27 @@ def _flat(t, dtype: str, count: int, device: int, what: str):
         return
     if _type_name(t.dtype) not in dtype or t.numel() < count or not t.is_contiguous():
         raise ValueError(f"{what}: {count} contiguous values of {dtype} expected")
-    if not _on(t, device):
+    if t.get_device() != device:   # -1 for a tensor that is on no GPU
         raise ValueError(f"{what}: not on the context's device")
 
 
 _Q4_WORDS = "torch.int32 torch.uint32 torch.uint8"
 _Q4_SCALES = "torch.bfloat16 torch.uint16 torch.int16 torch.uint8"
+_q4_words, _q4_scales = set(), set()   # the dtypes among them that calls have had
 
 
-def _q4_table(t, types: str, size: int, device: int, what: str, _held={}):
-    """A contiguous CUDA tensor of `size` bytes or more in one of `types`."""
-    held = _held.get((t.dtype, types))
-    if held is None:
-        held = _held.setdefault((t.dtype, types), str(t.dtype) in types.split())
-    if held and t.nbytes >= size and t.is_contiguous() and t.get_device() == device:
-        return
-    if not _on(t, device):
-        raise ValueError(f"q4_gemv_lora {what}: not on the context's device")
-    raise ValueError(f"q4_gemv_lora {what}: {size} contiguous bytes of {types} expected")
+def _q4_tables(packed, scales, biases, values: int, device: int):
+    """Contiguous CUDA tensors that hold `values` nibbles, and bf16 scales and
+    biases for every 64 of them.  q4_gemv_lora asks the same in one expression
+    and comes here where that fails or a dtype is new."""
+    for what, t, types, met, size in (("packed", packed, _Q4_WORDS, _q4_words, values >> 1),
+                                      ("scales", scales, _Q4_SCALES, _q4_scales, values >> 5),
+                                      ("biases", biases, _Q4_SCALES, _q4_scales, values >> 5)):
+        if str(t.dtype) not in types.split() or t.nbytes < size or not t.is_contiguous():
+            raise ValueError(f"q4_gemv_lora {what}: {size} contiguous bytes of {types} expected")
+        if t.get_device() != device:
+            raise ValueError(f"q4_gemv_lora {what}: not on the context's device")
+        met.add(t.dtype)
 
 
 class Routing:
@@ -259,10 +258,13 @@ class Context:
         (int32, negative: none) of the table `lora`; x and y rows of one type
         (fp32, bf16 or fp16), which may be strided.  W: words (or bytes) of eight
         nibbles, scales and biases in bf16 (or its bits) per group of 64."""
-        size = out_dim * in_dim
-        _q4_table(packed, _Q4_WORDS, size >> 1, self.device, "packed")
-        _q4_table(scales_bf16, _Q4_SCALES, size >> 5, self.device, "scales")
-        _q4_table(biases_bf16, _Q4_SCALES, size >> 5, self.device, "biases")
+        n, dev = out_dim * in_dim, self.device
+        if not (packed.dtype in _q4_words and packed.nbytes >= n >> 1 and packed.is_contiguous()
+                and packed.get_device() == dev and scales_bf16.dtype in _q4_scales
+                and scales_bf16.nbytes >= n >> 5 and scales_bf16.is_contiguous() and scales_bf16.get_device() == dev
+                and biases_bf16.dtype in _q4_scales and biases_bf16.nbytes >= n >> 5
+                and biases_bf16.is_contiguous() and biases_bf16.get_device() == dev):
+            _q4_tables(packed, scales_bf16, biases_bf16, n, dev)
         code, xs = _rows(x, in_dim, tokens, self.device, "q4_gemv_lora x")
         ycode, ys = _rows(y, out_dim, tokens, self.device, "q4_gemv_lora y")
         if ycode != code:
