@@ -6,7 +6,7 @@
 // an adapter count.  Rows are fp32, bf16 or fp16.
 //
 // Up to 4 tokens: lora_decode_kernel (W x on CUDA cores, v[t] = gain A_a x[t]
-// in every block, then B_a v).  One token 2048 -> 512 of rank 16: 6.9 us a
+// in every block, then B_a v).  One token 2048 -> 512 of rank 16: 7.7 us a
 // call, of which the launch is the larger part.
 //
 // Decode batches (up to 256 tokens while the products are fewer than what
@@ -30,9 +30,9 @@
 // requests needs no sorting and no second pass over y.  v is computed by tf32
 // matrix products (x as hi + lo for fp32 rows), once for every distinct adapter
 // of a tile of tokens, in the prep kernel or, from 4096 tokens on, in
-// lora_v_kernel.  4096 bf16 tokens 2048 x 2048, 8 adapters of rank 16: 78 us
-// (of these v 15, operands 14, products 61 with cold caches); 6001 fp32 tokens,
-// 12 adapters of rank 64: 244 us (55, 28, 186).
+// lora_v_kernel.  4096 bf16 tokens 2048 x 2048, 8 adapters of rank 16: 83 us (63
+// without adapters; one after the other with cold caches v takes 17, operands 18,
+// products 66); 6001 fp32 tokens, 12 adapters of rank 64: 248 us (56, 31, 191).
 //
 // What rounds there: fp32 rows hold 22 bits of x (products to about 2^-22) and
 // sum 16 products per step; the tensor core's accumulation drops what lies below
@@ -657,19 +657,14 @@ __device__ __forceinline__ void prep_row(const LoraArgs& a, long long t) {
     sum += __shfl_xor_sync(mask, sum, 1);
     sum += __shfl_xor_sync(mask, sum, 2);
     sum += __shfl_xor_sync(mask, sum, 4);
-    if ((threadIdx.x & 7) == 0) {
+    // the first of them store it, a column (or plane) each
+    const int part = threadIdx.x & 7;
+    if (part < (PB == 2 ? 2 : 3)) {
       const int grp = i >> 6;
       const float x = sum * (1.0f / 64.0f);  // stays below 2^15; the biases carry the 64
       const __half h = __float2half_rn(x), l = __float2half_rn(x - __half2float(h));
-      if constexpr (PB == 2) {
-        unsigned char* gat = column_at(grp);
-        *reinterpret_cast<__half*>(gat) = h;
-        *reinterpret_cast<__half*>(gat + (size_t)a.NT * 128) = l;
-      } else {
-        *reinterpret_cast<__half*>(column_at(3 * grp)) = h;
-        *reinterpret_cast<__half*>(column_at(3 * grp + 1)) = l;
-        *reinterpret_cast<__half*>(column_at(3 * grp + 2)) = h;
-      }
+      unsigned char* gat = PB == 2 ? column_at(grp) + (size_t)part * a.NT * 128 : column_at(3 * grp + part);
+      *reinterpret_cast<__half*>(gat) = part == 1 ? l : h;
     }
   };
 #pragma unroll
@@ -1261,10 +1256,13 @@ constexpr size_t kLgQTile = (size_t)32 * kLgQPitch;
 
 // Both operands are in shared memory, which leaves tensor memory to two buffers
 // of 256 tokens' sums, so that a tile's epilogue runs beside the next tile's
-// products.  What bounds the kernel is shared memory: 16384 bf16 tokens 2048 x
-// 2048 take 275 us for the whole call, 213 without adapters and stores of y,
-// 181 without the conversion of the weights; the matrix steps alone would take
-// 64 of them.
+// products.  By what a stage moves through shared memory (operands of the matrix
+// unit, Q4 tiles, converted weights: 800 clocks for 256 tokens) the products of
+// 4096 bf16 tokens 2048 x 2048 need 30 us, by their matrix steps 16; they take 66
+// on their own (the unit 32 % active, 0.39 instructions per scheduler and clock, 29
+// % of the load/store wavefronts), so what a stage waits for is the way of the
+// weights: Q4 tile, conversion, operand.  16384 tokens: 285 us the whole call, 214
+// without adapters.
 template <bool F32>
 struct LgCfg {
   static constexpr int PL = F32 ? 2 : 1;        // planes of x
@@ -1273,11 +1271,11 @@ struct LgCfg {
   static constexpr int NV = F32 ? 3 : 2;        // bf16 planes of v
 };
 // Stages that a block of adapters takes in a tile of `tokens`: the nv planes of
-// v, as many a stage as fit beside each other, and for fp16 adapters (`lo`) those
-// that the lo part of B meets, all but the last.
+// v in one where they fit beside each other (256 rows), else in two; and for fp16
+// adapters (`lo`) one for the low part of B, which meets all planes but the last.
+// Both hold for 3 planes of up to 128 tokens and 2 of up to 256.
 __host__ __device__ constexpr int lora_passes(int nv, int tokens, bool lo) {
-  const int per = 256 / tokens < nv ? 256 / tokens : nv;
-  return (nv + per - 1) / per + (lo ? (nv - 1 + per - 1) / per : 0);
+  return (nv * tokens <= 256 ? 1 : 2) + (lo ? 1 : 0);
 }
 // A converter warp's first block of adapters in a tile, brought ahead: the
 // pieces, and the entries of its threads' tokens.
@@ -1475,7 +1473,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
       for (int tile = first_tile; tile < tiles && ok; tile += step) {
         const int npad = (tokens_of(tile) + 15) & ~15;
         const uint32_t idf = idesc16(kLgM, npad, false), idb = idesc16(kLgM, npad, true);
-        const int vpl = v_planes(npad), hi = lora_passes(C::NV, npad, false), passes = lora_passes(C::NV, npad, BLO);
+        const int vpl = v_planes(npad), passes = lora_passes(C::NV, npad, BLO);
         const int total = stages_of(npad, ng);
         ng = pieces_at(tile + step);
         for (int c = 0; c < total; ++c, ++os) {
@@ -1505,9 +1503,8 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
             if (F32 && (k_lo + c < nk || ((k_lo + c - nk) & 1) == 0)) issue((uint32_t)C::NMAX * 128, idf);
           } else {
             const int pass = (c - nkm) % passes;
-            const bool lo_part = BLO && pass >= hi;
-            const int p0 = (lo_part ? pass - hi : pass) * vpl;
-            const int planes = min(lo_part ? C::NV - 1 : C::NV, p0 + vpl) - p0;
+            const bool lo_part = BLO && pass == passes - 1;
+            const int planes = lo_part ? C::NV - 1 : min(vpl, C::NV - pass * vpl);
             for (int p = 0; p < planes; ++p) issue((uint32_t)(p * npad * 128), idb);
           }
           commit(&S.opempty[st]);
@@ -1638,7 +1635,7 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
         return true;
       };
       // ---- a stage of adapters: a block of 64 columns, four pieces of 16 rows ----
-      const int vpl = v_planes(npad), hi = lora_passes(C::NV, npad, false), passes = lora_passes(C::NV, npad, BLO);
+      const int vpl = v_planes(npad), passes = lora_passes(C::NV, npad, BLO);
       auto block_of = [&](int c) { return rank_c + (c - nkm) / passes * split; };
       const int c_first = nkm + ((nkm ^ grp) & 1);   // this group's first such stage
       LgAhead& ahead = S.ahead[warp - 2];
@@ -1663,9 +1660,9 @@ __global__ void __launch_bounds__(kLgThreads, 1) lora_gemm_kernel(const __grid_c
         const uint32_t oc = os + (uint32_t)c;
         const int st = (int)(oc % kLgRO);
         const int blk = block_of(c), pass = (c - nkm) % passes;
-        const bool lo_part = BLO && pass >= hi;
-        const int p0 = (lo_part ? pass - hi : pass) * vpl;
-        const int planes = min(lo_part ? C::NV - 1 : C::NV, p0 + vpl) - p0;
+        const bool lo_part = BLO && pass == passes - 1;
+        const int p0 = lo_part ? 0 : pass * vpl;
+        const int planes = lo_part ? C::NV - 1 : min(vpl, C::NV - p0);
         const bool here = c == c_first;
         if (here) {
           asm volatile("cp.async.wait_all;" ::: "memory");
