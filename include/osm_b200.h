@@ -200,17 +200,26 @@ typedef struct {
  * without the second term where a is negative; an index of `count` or more is
  * taken as none and sets status bit 8.  lora (and adapter_dev) NULL: the
  * projection alone.  W as for osm_q4_gemv with bf16 scale and bias; group 64,
- * in_dim a multiple of 64, any out_dim, any number of tokens (the context's
- * max_tokens does not bound it).  x and y are rows of one type, x_stride and
- * y_stride elements apart (0: packed); rows and values behind the last one
- * are neither read nor written, and y must not overlap x.  Sums are held in
- * fp32, y is rounded once; a token's row depends on no other token's row and
- * no other adapter.  A row of x with a NaN or an infinity gives non-finite
- * values in its own y.  Workspace is the context's, at most
- * 256 MB a call beside a fifth of W: the first four streams keep a block each,
- * calls on others take and return memory in the stream's order, and a captured
- * call carries its own in the graph, so calls on two streams do not meet and a
- * stream may be destroyed right behind its calls. */
+ * in_dim a multiple of 64, in_dim and out_dim up to 2^20, up to 2^24 tokens (the
+ * context's max_tokens does not bound them).  x and y are rows of one type,
+ * x_stride and y_stride elements apart (0: packed); rows and values behind the
+ * last one are neither read nor written, and the memory from y's first to its
+ * last value must not overlap x's.
+ * Sums are held in fp32 and y is rounded once.  Calls of more than 256 tokens or
+ * 1e9 products hold the values of fp32 rows, the weights' biases and the sums of x
+ * that meet these in 22 bits or more, and A_a x[t] of 16-bit rows in 16 bits.  No
+ * value of another token's row or another adapter enters a token's row, not even
+ * one that is not finite; but the order of its sums, and so its last bits, depend
+ * on the batch that it is in (its size, and the other adapters of a tile).  The
+ * same call gives the same bits.  A row of x with a NaN or an infinity gives
+ * non-finite values in its own y.
+ * Workspace is the context's, at most 256 MB a call (or what 256 tokens need)
+ * beside a fifth of W: the first four streams keep a block each, calls on others
+ * take and return memory in the stream's order, so calls on two streams do not
+ * meet and a stream may be destroyed right behind its calls.  A captured call
+ * has its own memory in the graph, which holds an allocation and a release node
+ * then: such a graph cannot be a child of another one, nor be instantiated twice
+ * at a time. */
 int osm_q4_gemv_lora(osm_context* ctx, const uint32_t* packed_dev,
                      const uint16_t* scales_bf16_dev,
                      const uint16_t* biases_bf16_dev, uint32_t out_dim,

@@ -6,7 +6,7 @@
 // an adapter count.  Rows are fp32, bf16 or fp16.
 //
 // Up to 4 tokens: lora_decode_kernel (W x on CUDA cores, v[t] = gain A_a x[t]
-// in every block, then B_a v).  One token 2048 -> 512 of rank 16: 7.7 us a
+// in every block, then B_a v).  One token 2048 -> 512 of rank 16: 7.5 us a
 // call, of which the launch is the larger part.
 //
 // Decode batches (up to 256 tokens while the products are fewer than what
@@ -30,9 +30,9 @@
 // requests needs no sorting and no second pass over y.  v is computed by tf32
 // matrix products (x as hi + lo for fp32 rows), once for every distinct adapter
 // of a tile of tokens, in the prep kernel or, from 4096 tokens on, in
-// lora_v_kernel.  4096 bf16 tokens 2048 x 2048, 8 adapters of rank 16: 83 us (63
-// without adapters; one after the other with cold caches v takes 17, operands 18,
-// products 66); 6001 fp32 tokens, 12 adapters of rank 64: 248 us (56, 31, 191).
+// lora_v_kernel.  4096 bf16 tokens 2048 x 2048, 8 adapters of rank 16: 80 us (62
+// without adapters; one after the other with cold caches v takes 17, operands 16,
+// products 64); 6001 fp32 tokens, 12 adapters of rank 64: 249 us (53, 28, 188).
 //
 // What rounds there: fp32 rows hold 22 bits of x (products to about 2^-22) and
 // sum 16 products per step; the tensor core's accumulation drops what lies below
@@ -1258,7 +1258,7 @@ constexpr size_t kLgQTile = (size_t)32 * kLgQPitch;
 // of 256 tokens' sums, so that a tile's epilogue runs beside the next tile's
 // products.  By what a stage moves through shared memory (operands of the matrix
 // unit, Q4 tiles, converted weights: 800 clocks for 256 tokens) the products of
-// 4096 bf16 tokens 2048 x 2048 need 30 us, by their matrix steps 16; they take 66
+// 4096 bf16 tokens 2048 x 2048 need 30 us, by their matrix steps 16; they take 64
 // on their own (the unit 32 % active, 0.39 instructions per scheduler and clock, 29
 // % of the load/store wavefronts), so what a stage waits for is the way of the
 // weights: Q4 tile, conversion, operand.  16384 tokens: 285 us the whole call, 214

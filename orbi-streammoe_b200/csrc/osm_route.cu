@@ -29,7 +29,7 @@
 // experts; these are ranked against each other, at most two per lane.
 //
 // Small batches are bound by the launch (one token of 512 to 4096 tokens of 512
-// experts: 6.6 us a call), large ones by instructions: 16384 fp32 tokens of 256
+// experts: 6 to 6.5 us a call), large ones by instructions: 16384 fp32 tokens of 256
 // experts in 8 groups with a bias take 21 to 27 us, about 1000 warp instructions a
 // token at 0.75 per clock, where their 18 MB would take 2.7.  The whole in 64
 // bits, expert by expert in shared memory with top_k rounds of an argmax, took
