@@ -1144,9 +1144,14 @@ int osm_context_destroy(osm_context* ctx) {
   cudaStreamSynchronize(ctx->stream);
   if (ctx->sc.base) cudaFree(ctx->sc.base);
   for (void* p : ctx->retired) cudaFree(p);
-  for (const auto& w : ctx->works)
-    if (w.base) cudaFree(w.base);
-  if (ctx->work_pool) cudaMemPoolDestroy(ctx->work_pool);
+  if (ctx->work_pool) {
+    // memory of a pool is released at once, so no stream may still use its block
+    // (should the device not be able to wait, the blocks are left)
+    if (cudaDeviceSynchronize() == cudaSuccess)
+      for (const auto& w : ctx->works)
+        if (w.base) cudaFree(w.base);
+    cudaMemPoolDestroy(ctx->work_pool);
+  }
   if (ctx->status_blk) cudaFree(ctx->status_blk);
   for (const ProfRec& r : ctx->recs) {
     cudaEventDestroy(r.a);

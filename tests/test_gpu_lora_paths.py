@@ -354,3 +354,73 @@ def test_sublayer_of_many_requests(torch, T):  # noqa: F811
     out.fill_(-7)
     graph.replay()
     verify()
+
+
+def test_context_destroyed_behind_its_calls(torch):  # noqa: F811
+    """A context may go while the calls of several streams still run."""
+    import osm_b200 as osm
+
+    cases = [Case(torch, T, 2048, 1024, n=9, rank=64, dtype=d, seed=i) for i, (T, d) in
+             enumerate([(6000, "fp32"), (5000, "bf16"), (900, "fp16")])]
+    want = []
+    first = osm.Context(0, max_tokens=4)
+    for c in cases:
+        first.set_stream(torch.cuda.current_stream().cuda_stream)
+        want.append(c.run(first).clone())
+    torch.cuda.synchronize()
+    first.close()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(3):
+        for c in cases:
+            c.yw.fill_(-7)
+        torch.cuda.synchronize()
+        ctx = osm.Context(0, max_tokens=4)
+        for c, s in zip(cases, streams):
+            ctx.set_stream(s.cuda_stream)
+            for _ in range(10):
+                c.run(ctx)
+        ctx.reset_stream()
+        ctx.close()
+        torch.cuda.synchronize()
+        for c, w in zip(cases, want):
+            assert torch.equal(c.y, w)
+
+
+FIRST_CALL = """
+import sys
+sys.path[:0] = {paths!r}
+import torch
+import osm_b200 as osm
+from test_gpu_lora import Case
+ctx = osm.Context(0, max_tokens=4)
+cases = [Case(torch, T, K, 256, n=5, rank=40, dtype=d, half=h, seed=i) for i, (T, K, d, h) in enumerate(
+    [(3, 8192, "fp32", "bf16"), (4, 512, "fp32", "fp16"), (90, 512, "fp32", "fp16"), (200, 768, "bf16", "bf16"),
+     (700, 512, "fp32", "fp16"), (4200, 320, "bf16", "fp16")])]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    for c in cases:
+        c.run(ctx)
+for c in cases:
+    c.yw.fill_(-7)
+g.replay()
+torch.cuda.synchronize()
+got = [c.y.clone() for c in cases]
+ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+for c, y in zip(cases, got):
+    c.check(torch, ctx)
+    assert torch.equal(c.y, y)
+print("PASS")
+"""
+
+
+def test_first_calls_of_a_process_are_captured(torch):  # noqa: F811
+    """Kernels that were never launched before, and ask for their shared memory at
+    their first launch, may have it under capture."""
+    import subprocess
+    import sys
+
+    paths = [p for p in sys.path if p]
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(paths=paths)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "PASS" in r.stdout, (r.stdout[-2000:], r.stderr[-2000:])
