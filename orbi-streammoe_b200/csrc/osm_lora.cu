@@ -2154,11 +2154,11 @@ size_t shape(LoraArgs& a, int sms, unsigned char* base) {
     const long long most = a.tokens < a.count ? a.tokens : a.count;
     // v: tiles of 16 tokens in the prep kernel while a tile's adapters are worth
     // blocks of their own, a kernel of its own where a prompt's tokens share them
-    // (2500 bf16 tokens 2048 x 2048, 8 adapters of rank 16: 72 us against 75; 3500,
-    // every token another of 64: 235 against 329; 3500 fp32 tokens 2048 -> 768, 8
-    // adapters of rank 64: 103 against 102; above, prompts decide: 4096 tokens of 8
-    // requests 85 against 78, 6000 fp32 tokens of 12 of rank 64 255 against 238,
-    // though 6000 tokens that each take another of 64 would gain, 387 against 554)
+    // (2500 bf16 tokens 2048 x 2048, 8 adapters of rank 16: 72 us against 74; 3500,
+    // every token another of 64: 245 against 338; 3500 fp32 tokens 2048 -> 768, 8
+    // adapters of rank 64: 98 against 96; above, prompts decide: 4096 tokens of 8
+    // requests 86 against 80, 6000 fp32 tokens of 12 of rank 64 260 against 243,
+    // though 6000 tokens that each take another of 64 would gain, 385 against 548)
     a.v_self = v_by_self(a);
     if (a.v_self || v_by_rows(a)) {
       // no tiles
