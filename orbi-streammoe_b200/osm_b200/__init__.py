@@ -168,6 +168,24 @@ def expert_layout(hidden: int, inter: int, group: int = 64) -> ExpertLayout:
     return L
 
 
+class _Life:
+    """A library object that others use: destroyed when its own Python object is
+    closed and the last of theirs has been.  Counted by hand, because a collected
+    cycle finalises its objects in any order."""
+
+    def __init__(self, destroy, user_of: "_Life | None" = None):
+        self.destroy, self.user_of, self.uses = destroy, user_of, 1
+        if user_of is not None:
+            user_of.uses += 1
+
+    def release(self):
+        self.uses -= 1
+        if self.uses == 0:
+            self.destroy()
+            if self.user_of is not None:
+                self.user_of.release()
+
+
 class Context:
     """One device, one stream, scratch for up to ``max_tokens`` rows."""
 
@@ -176,6 +194,8 @@ class Context:
         rc = lib().osm_context_create(device, max_tokens, C.byref(self.h))
         if rc:
             raise OsmError(rc, "context creation failed")
+        h = self.h
+        self.life = _Life(lambda: lib().osm_context_destroy(h))
         self.device = device
         self.max_tokens = max_tokens
 
@@ -185,9 +205,10 @@ class Context:
             raise OsmError(rc, f"{what}: {msg}" if what else msg)
 
     def close(self):
+        """The context goes once its slabs, layers and plans are closed too."""
         if self.h:
-            lib().osm_context_destroy(self.h)
             self.h = C.c_void_p()
+            self.life.release()
 
     def __del__(self):
         try:
@@ -327,12 +348,14 @@ class Slab:
         self.layout = layout
         self.h = C.c_void_p()
         ctx.check(lib().osm_slab_create(ctx.h, C.byref(layout), slots, C.byref(self.h)), "slab")
+        h = self.h
+        self.life = _Life(lambda: lib().osm_slab_destroy(h), ctx.life)
         self.slots = slots
 
     def close(self):
         if self.h:
-            lib().osm_slab_destroy(self.h)
             self.h = C.c_void_p()
+            self.life.release()
 
     def __del__(self):
         try:
@@ -392,13 +415,16 @@ class Layer:
         d.norm_eps = norm_eps
         self.h = C.c_void_p()
         ctx.check(lib().osm_layer_create(ctx.h, C.byref(d), C.byref(self.h)), "layer")
+        h = self.h
+        self.life = _Life(lambda: lib().osm_layer_destroy(h), ctx.life)
         self.hidden, self.experts, self.top_k = H, E, top_k
         self.has_shared = shared_slot is not None
 
     def close(self):
+        """The layer goes once its plans are closed too."""
         if self.h:
-            lib().osm_layer_destroy(self.h)
             self.h = C.c_void_p()
+            self.life.release()
 
     def __del__(self):
         try:
@@ -519,6 +545,8 @@ class Plan:
         layer.ctx.check(lib().osm_plan_create(layer.h, tokens, _ptr(x), _ptr(out), _ptr(ids),
                                               _ptr(weights), _ptr(x_host), _ptr(out_host), flags,
                                               C.byref(self.h)), "plan")
+        h = self.h
+        self.life = _Life(lambda: lib().osm_plan_destroy(h), layer.life)
         self.kernels = lib().osm_plan_kernels(self.h)
 
     def launch(self):
@@ -534,8 +562,8 @@ class Plan:
 
     def close(self):
         if self.h:
-            lib().osm_plan_destroy(self.h)
             self.h = C.c_void_p()
+            self.life.release()
 
     def __del__(self):
         try:
